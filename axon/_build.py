@@ -61,6 +61,9 @@ def build(verbose=False):
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         f"--offload-arch={ARCH}",
         "-Wall", "-Wno-unused-function",
+        # No packed FP32 arithmetic in device code: hipcc forms it by itself
+        # from scalar float code, and some forms are not reliable on gfx950.
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     ]
     torch_defs = [
         "-D_GLIBCXX_USE_CXX11_ABI=1",
