@@ -166,13 +166,13 @@ __global__ void adam_kernel(const OptChunk* __restrict__ chunks, float lr,
 // for Deep Learning" (LAMB).
 
 // 64-lane sum via one f32 MFMA (v_mfma_f32_16x16x4_f32): lane l holds
-// A[l&15][l>>4] and B[l>>4][l&15]; with B=1 the D row sums A over k, i.e.
+// A[l&15][l>>4] and B[l>>4][l&15]; with A=1 each row of D sums B over k, i.e.
 // lane groups {i, i+16, i+32, i+48} — a 64->16 reduction on the matrix
 // core — then 4 DS swizzles finish 16->1.
 __device__ __forceinline__ float wave_sum_mfma(float x) {
   using f32x4 = __attribute__((ext_vector_type(4))) float;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x, 1.0f, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, x, acc, 0, 0, 0);
   // Lane l now holds D[row=(l>>4)*4+reg][col=l&15]; every row of D equals
   // the same 16 column sums, so take reg 0 and butterfly the 16 columns.
   float s = acc[0];
