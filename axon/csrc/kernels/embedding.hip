@@ -1,0 +1,410 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+//   fwd: y[n] = scale * W[id[n]]                       (rows of D values)
+//   bwd: dW[v] = scale * sum_{n: id[n] = v} dy[n]      (zeros where no n)
+//
+// Both are bound by memory: N*D values read and written forward, N*D read
+// and V*D written backward. The backward pass never adds with atomics, so it
+// gives the same bits each time: the tokens are sorted by (id, position) and
+// each id's rows are then summed in the order of their positions.
+#include <algorithm>
+
+#include "kernels.h"
+#include "lm_util.h"
+
+namespace axon {
+
+namespace {
+
+using namespace lm;
+
+constexpr int kThreads = 256;
+
+// ------------------------------------------------------------------ forward
+//
+// A group of `lanes` lanes copies up to kFwdVecs 16-byte vectors of one row;
+// wide rows are spread over gridDim.y. An id outside [0, V) gives a row of
+// NaN: the kernel reads nothing for it, and the caller sees it in the loss.
+
+constexpr int kFwdVecs = 4;
+
+template <typename T, typename I>
+__global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
+    const I* __restrict__ ids, const T* __restrict__ w, T* __restrict__ y,
+    int64_t n, int64_t vocab, int64_t dim, int64_t wstride, float scale,
+    int lanes) {
+  constexpr int V = kVec<T>;
+  const int64_t row =
+      static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) +
+      threadIdx.x / lanes;
+  if (row >= n) return;
+  const int64_t c0 =
+      (static_cast<int64_t>(blockIdx.y) * kFwdVecs * lanes +
+       threadIdx.x % lanes) * V;
+  const int64_t id = static_cast<int64_t>(ids[row]);
+  const bool known = id >= 0 && id < vocab;
+  const T* src = w + (known ? id * wstride : 0);
+  T* dst = y + row * dim;
+  const float s = known ? scale : __builtin_nanf("");
+  u32x4 r[kFwdVecs];
+#pragma unroll
+  for (int k = 0; k < kFwdVecs; ++k) {
+    const int64_t c = c0 + static_cast<int64_t>(k) * lanes * V;
+    if (c + V <= dim) r[k] = known ? load16(src + c) : u32x4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int k = 0; k < kFwdVecs; ++k) {
+    const int64_t c = c0 + static_cast<int64_t>(k) * lanes * V;
+    if (c + V <= dim) {
+      float f[V];
+      unpack<T>(r[k], f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] *= s;
+      store16(dst + c, pack<T>(f));
+    } else {
+      for (int64_t i = c; i < dim; ++i)
+        dst[i] = static_cast<T>((known ? static_cast<float>(src[i]) : 0.f) * s);
+    }
+  }
+}
+
+// ----------------------------------------------------------- sorting tokens
+//
+// A key is id << 32 | position: keys differ from each other, so any way of
+// sorting them gives one order. Ids that take no part (padding, or outside
+// [0, V)) get the id V and end up behind all others.
+//
+// Tiles of kTile keys are sorted in LDS (bitonic); then runs are merged, up
+// to kMergeRuns at a time: a key's place in the merged run is its place in
+// its own run plus the number of smaller keys in each of the others, found by
+// bisection. That takes one launch for up to 32768 tokens, two up to 524288.
+
+constexpr int kTile = 2048;
+constexpr int kSortThreads = 1024;
+constexpr int kMergeRuns = 16;
+
+// The blocks behind the tiles' fill dW with zeros meanwhile: sorting is a
+// matter of latency on few CUs, filling one of bandwidth.
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
+    const I* __restrict__ ids, uint64_t* __restrict__ keys, int64_t n,
+    int64_t vocab, int64_t padding, int tiles, uint16_t* __restrict__ zeros,
+    int64_t nzeros) {
+  __shared__ uint64_t s[kTile];
+  if (static_cast<int>(blockIdx.x) >= tiles) {
+    const int64_t step =
+        static_cast<int64_t>(gridDim.x - tiles) * kSortThreads;
+    const int64_t at = static_cast<int64_t>(blockIdx.x - tiles) * kSortThreads +
+                       threadIdx.x;
+    u32x4* wide = reinterpret_cast<u32x4*>(zeros);
+    for (int64_t i = at; i < nzeros / 8; i += step) wide[i] = u32x4{0, 0, 0, 0};
+    if (at < nzeros % 8) zeros[nzeros / 8 * 8 + at] = 0;
+    return;
+  }
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
+  for (int i = threadIdx.x; i < kTile; i += kSortThreads) {
+    uint64_t key = ~0ull;
+    if (base + i < n) {
+      const int64_t id = static_cast<int64_t>(ids[base + i]);
+      const bool part = id >= 0 && id < vocab && id != padding;
+      key = static_cast<uint64_t>(part ? id : vocab) << 32 |
+            static_cast<uint32_t>(base + i);
+    }
+    s[i] = key;
+  }
+  __syncthreads();
+  for (int k = 2; k <= kTile; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int t = threadIdx.x; t < kTile / 2; t += kSortThreads) {
+        const int a = 2 * t - (t & (j - 1)), b = a + j;
+        const uint64_t x = s[a], y = s[b];
+        if ((x > y) == ((a & k) == 0)) {
+          s[a] = y;
+          s[b] = x;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  for (int i = threadIdx.x; i < kTile; i += kSortThreads)
+    if (base + i < n) keys[base + i] = s[i];
+}
+
+// Keys below `key` in the sorted run p[0..n).
+__device__ __forceinline__ int64_t count_below(const uint64_t* p, int64_t n,
+                                               uint64_t key) {
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (p[mid] < key)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kThreads) void embed_merge_kernel(
+    const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int64_t n,
+    int64_t run) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= n) return;
+  const uint64_t key = in[i];
+  const int64_t group = i / (run * kMergeRuns) * (run * kMergeRuns);
+  const int64_t mine = i / run * run;
+  int64_t place = group + (i - mine);
+  for (int r = 0; r < kMergeRuns; ++r) {
+    const int64_t start = group + r * run;
+    if (start >= n) break;
+    if (start != mine)
+      place += count_below(in + start, min(run, n - start), key);
+  }
+  out[place] = key;
+}
+
+// ------------------------------------------------------------ summing rows
+//
+// The sorted positions are cut into chunks of equal length, whatever the
+// tokens' frequencies: a wave sums one chunk over one slice of columns and
+// writes each id's row when the id changes. Rows of an id that crosses a
+// chunk's border go to fp32 partial sums (slot 0: the id came from the chunk
+// before; slot 1: it starts here and goes on), which a second kernel joins
+// in order.
+
+constexpr int kRowsAhead = 8;
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void embed_sum_kernel(
+    const uint64_t* __restrict__ keys, const T* __restrict__ dy,
+    T* __restrict__ dw, float* __restrict__ part, int64_t n, int64_t vocab,
+    int64_t dim, int chunk, int64_t nchunks, int slices, float scale) {
+  constexpr int V = kVec<T>;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) +
+                       (threadIdx.x >> 6);
+  const int64_t ci = unit / slices;
+  if (ci >= nchunks) return;
+  const int64_t c0 = (unit % slices) * 64 * V + lane * V;
+  const int64_t begin = ci * chunk;
+  const int64_t end = min(begin + chunk, n);
+  const int width = c0 >= dim ? 0 : static_cast<int>(min<int64_t>(V, dim - c0));
+
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  int64_t cur = static_cast<int64_t>(keys[begin] >> 32);
+  bool first = begin > 0 &&
+               static_cast<int64_t>(keys[begin - 1] >> 32) == cur;
+
+  auto flush = [&](bool goes_on) {
+    if (cur >= vocab || width == 0) return;
+    if (first || goes_on) {
+      float* p = part + (ci * 2 + (first ? 0 : 1)) * dim + c0;
+      for (int i = 0; i < V; ++i)
+        if (i < width) p[i] = acc[i];
+    } else {
+      T* p = dw + cur * dim + c0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] *= scale;
+      if (width == V) {
+        store16(p, pack<T>(acc));
+      } else {
+        for (int i = 0; i < V; ++i)
+          if (i < width) p[i] = static_cast<T>(acc[i]);
+      }
+    }
+  };
+
+  for (int64_t p0 = begin; p0 < end; p0 += kRowsAhead) {
+    u32x4 r[kRowsAhead];
+    int64_t id[kRowsAhead];
+#pragma unroll
+    for (int k = 0; k < kRowsAhead; ++k) {
+      id[k] = vocab;
+      r[k] = u32x4{0, 0, 0, 0};
+      if (p0 + k < end) {
+        const uint64_t key = keys[p0 + k];
+        id[k] = static_cast<int64_t>(key >> 32);
+        const T* src = dy + static_cast<int64_t>(key & 0xffffffffu) * dim + c0;
+        if (id[k] < vocab) {
+          if (width == V) {
+            r[k] = load16(src);
+          } else if (width > 0) {
+            T t[V] = {};
+            for (int i = 0; i < V; ++i)
+              if (i < width) t[i] = src[i];
+            __builtin_memcpy(&r[k], t, 16);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRowsAhead; ++k) {
+      if (p0 + k < end) {
+        if (id[k] != cur) {
+          flush(false);
+          first = false;
+          cur = id[k];
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        }
+        float f[V];
+        unpack<T>(r[k], f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += f[i];
+      }
+    }
+  }
+  flush(end < n && static_cast<int64_t>(keys[end] >> 32) == cur);
+}
+
+// One block joins one chunk's slot 1 with the slots 0 behind it, if an id
+// starts in that chunk and goes on: its four waves take every fourth chunk
+// and are summed in order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void embed_join_kernel(
+    const uint64_t* __restrict__ keys, const float* __restrict__ part,
+    T* __restrict__ dw, int64_t n, int64_t vocab, int64_t dim, int chunk,
+    float scale) {
+  const int64_t ci = blockIdx.x;
+  const int64_t begin = ci * chunk, end = begin + chunk;
+  if (end >= n) return;
+  const int64_t id = static_cast<int64_t>(keys[end] >> 32);
+  if (id >= vocab || static_cast<int64_t>(keys[end - 1] >> 32) != id) return;
+  // Starts it here? Else an earlier chunk joins it.
+  if (begin > 0 && static_cast<int64_t>(keys[begin] >> 32) == id &&
+      static_cast<int64_t>(keys[begin - 1] >> 32) == id)
+    return;
+  const uint64_t after = static_cast<uint64_t>(id + 1) << 32;
+  const int64_t last =
+      (end + count_below(keys + end, n - end, after) - 1) / chunk;
+  __shared__ float s[kThreads / 64][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t c = static_cast<int64_t>(blockIdx.y) * 64 + lane;
+  float acc = 0.f;
+  if (c < dim) {
+    if (wave == 0) acc = part[(ci * 2 + 1) * dim + c];
+#pragma unroll 4
+    for (int64_t k = ci + 1 + wave; k <= last; k += kThreads / 64)
+      acc += part[k * 2 * dim + c];
+  }
+  s[wave][lane] = acc;
+  __syncthreads();
+  if (wave == 0 && c < dim) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) sum += s[w][lane];
+    dw[id * dim + c] = static_cast<T>(sum * scale);
+  }
+}
+
+struct SumPlan {
+  int chunk;
+  int64_t nchunks;
+  int slices;
+};
+
+// Chunks are as long as still leaves about 4096 waves (4 for each SIMD), and
+// 8 to 256 tokens: a short chunk keeps few loads in flight, a long one leaves
+// CUs idle.
+SumPlan sum_plan(int64_t n, int64_t dim, int vec) {
+  SumPlan p;
+  p.slices = static_cast<int>((dim + 64 * vec - 1) / (64 * vec));
+  p.chunk = 8;
+  while (p.chunk < 256 && n / p.chunk * p.slices > 4096) p.chunk *= 2;
+  p.nchunks = (n + p.chunk - 1) / p.chunk;
+  return p;
+}
+
+template <typename T, typename I>
+void bwd(const I* ids, const T* dy, T* dw, uint64_t* keys, float* part,
+         int64_t n, int64_t vocab, int64_t dim, int64_t padding, float scale,
+         hipStream_t stream) {
+  const int tiles = static_cast<int>((n + kTile - 1) / kTile);
+  const int64_t nzeros = vocab * dim * static_cast<int64_t>(sizeof(T) / 2);
+  const int fill = static_cast<int>(std::min<int64_t>(
+      1024, (nzeros / 8 + kSortThreads) / kSortThreads));
+  hipLaunchKernelGGL(embed_sort_kernel<I>, dim3(tiles + fill),
+                     dim3(kSortThreads), 0, stream, ids, keys, n, vocab,
+                     padding, tiles, reinterpret_cast<uint16_t*>(dw), nzeros);
+  if (n == 0) return;
+  uint64_t* other = keys + n;
+  for (int64_t run = kTile; run < n; run *= kMergeRuns) {
+    hipLaunchKernelGGL(embed_merge_kernel,
+                       dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, stream, keys, other, n, run);
+    std::swap(keys, other);
+  }
+  const SumPlan p = sum_plan(n, dim, kVec<T>);
+  const int64_t units = p.nchunks * p.slices;
+  hipLaunchKernelGGL(embed_sum_kernel<T>,
+                     dim3(static_cast<unsigned>((units + 3) / 4)),
+                     dim3(kThreads), 0, stream, keys, dy, dw, part, n, vocab,
+                     dim, p.chunk, p.nchunks, p.slices, scale);
+  if (p.nchunks > 1)
+    hipLaunchKernelGGL(embed_join_kernel<T>,
+                       dim3(static_cast<unsigned>(p.nchunks - 1),
+                            static_cast<unsigned>((dim + 63) / 64)),
+                       dim3(kThreads), 0, stream, keys, part, dw, n, vocab,
+                       dim, p.chunk, scale);
+}
+
+template <typename T, typename I>
+void fwd(const I* ids, const T* w, T* y, int64_t n, int64_t vocab, int64_t dim,
+         int64_t wstride, float scale, hipStream_t stream) {
+  int lanes = 1;
+  while (lanes < 64 && lanes * kVec<T> < dim) lanes *= 2;
+  const int rows = kThreads / lanes;
+  const int64_t cols = static_cast<int64_t>(lanes) * kVec<T> * kFwdVecs;
+  hipLaunchKernelGGL((embed_fwd_kernel<T, I>),
+                     dim3(static_cast<unsigned>((n + rows - 1) / rows),
+                          static_cast<unsigned>((dim + cols - 1) / cols)),
+                     dim3(kThreads), 0, stream, ids, w, y, n, vocab, dim,
+                     wstride, scale, lanes);
+}
+
+}  // namespace
+
+int64_t embed_part_floats(int64_t n, int64_t dim, int elem_size) {
+  const SumPlan p = sum_plan(n, dim, 16 / elem_size);
+  return p.nchunks * 2 * dim;
+}
+
+void launch_embed_fwd(int dtype, bool ids64, const void* ids, const void* w,
+                      void* y, int64_t n, int64_t vocab, int64_t dim,
+                      int64_t wstride, float scale, hipStream_t stream) {
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (ids64)
+      fwd(static_cast<const int64_t*>(ids), static_cast<const T*>(w),
+          static_cast<T*>(y), n, vocab, dim, wstride, scale, stream);
+    else
+      fwd(static_cast<const int32_t*>(ids), static_cast<const T*>(w),
+          static_cast<T*>(y), n, vocab, dim, wstride, scale, stream);
+  };
+  if (dtype == kFloat) go(float{});
+  if (dtype == kHalf) go(_Float16{});
+  if (dtype == kBF16) go(__bf16{});
+}
+
+void launch_embed_bwd(int dtype, bool ids64, const void* ids, const void* dy,
+                      void* dw, uint64_t* keys, float* part, int64_t n,
+                      int64_t vocab, int64_t dim, int64_t padding, float scale,
+                      hipStream_t stream) {
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (ids64)
+      bwd(static_cast<const int64_t*>(ids), static_cast<const T*>(dy),
+          static_cast<T*>(dw), keys, part, n, vocab, dim, padding, scale,
+          stream);
+    else
+      bwd(static_cast<const int32_t*>(ids), static_cast<const T*>(dy),
+          static_cast<T*>(dw), keys, part, n, vocab, dim, padding, scale,
+          stream);
+  };
+  if (dtype == kFloat) go(float{});
+  if (dtype == kHalf) go(_Float16{});
+  if (dtype == kBF16) go(__bf16{});
+}
+
+}  // namespace axon

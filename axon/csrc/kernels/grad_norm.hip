@@ -1,0 +1,206 @@
+// Norm over all gradients, and the gradients scaled by it:
+//
+//   r = (sum g^2)^(1/2), sum |g| or max |g| over all tensors
+//   c = min(1, max_norm / (r + 1e-6));  g <- c g
+//
+// Bound by memory: the gradients are read once for the norm, and read and
+// written once more where c < 1 (a norm within the bound leaves them alone).
+// Sums are in 64 bits: a norm up to the largest fp32 value comes out finite,
+// small gradients do not vanish when squared. No atomics: block b takes
+// chunks b, b + grid, ... and its partial sum has a place of its own, so the
+// same gradients give the same bits.
+#include <algorithm>
+
+#include "grad_norm.h"
+#include "lm_util.h"
+
+namespace axon {
+
+namespace {
+
+using namespace lm;
+
+constexpr int kThreads = 256;
+constexpr int kMaxBlocks = 2048;  // 8 blocks of 4 waves on each CU
+
+struct Sum {  // type 1 and 2
+  static __device__ double join(double a, double b) { return a + b; }
+};
+struct Most {  // type 0: NaN wins
+  static __device__ double join(double a, double b) {
+    return (b > a || b != b) ? b : a;
+  }
+};
+
+template <int kType>
+__device__ __forceinline__ double add(double acc, float f) {
+  const double d = static_cast<double>(f);
+  if (kType == 2) return fma(d, d, acc);
+  if (kType == 1) return acc + fabs(d);
+  return Most::join(acc, fabs(d));
+}
+
+template <typename J>
+__device__ double block_join(double v) {
+  __shared__ double lds[kThreads / 64];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = J::join(v, __shfl_xor(v, off, 64));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = lds[0];
+  for (int w = 1; w < kThreads / 64; ++w) v = J::join(v, lds[w]);
+  return v;
+}
+
+// The tensor that chunk c belongs to: the last one with first[i] <= c.
+__device__ __forceinline__ int tensor_of(const GradTable& t, int c) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= c)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T, int kType>
+__global__ __launch_bounds__(kThreads) void grad_partial_kernel(
+    const GradTable t, double* __restrict__ partial) {
+  constexpr int V = kVec<T>;
+  constexpr int kAhead = 4;
+  double acc = 0.0;
+  const int chunks = t.first[t.count];
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int i = tensor_of(t, c);
+    const int64_t begin = static_cast<int64_t>(c - t.first[i]) * kGradChunk;
+    const T* p = static_cast<const T*>(t.ptr[i]) + begin;
+    const int len = static_cast<int>(min(kGradChunk, t.n[i] - begin));
+    const int full = len / V;
+    int k = threadIdx.x;
+    for (; k + (kAhead - 1) * kThreads < full; k += kAhead * kThreads) {
+      u32x4 r[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) r[a] = load16(p + (k + a * kThreads) * V);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        float f[V];
+        unpack<T>(r[a], f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc = add<kType>(acc, f[e]);
+      }
+    }
+    for (; k < full; k += kThreads) {
+      float f[V];
+      unpack<T>(load16(p + k * V), f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc = add<kType>(acc, f[e]);
+    }
+    for (int j = full * V + threadIdx.x; j < len; j += kThreads)
+      acc = add<kType>(acc, static_cast<float>(p[j]));
+  }
+  using J = std::conditional_t<kType == 0, Most, Sum>;
+  acc = block_join<J>(acc);
+  if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+template <int kType>
+__global__ __launch_bounds__(kThreads) void grad_finish_kernel(
+    const double* __restrict__ partial, int blocks, float max_norm,
+    float* __restrict__ out) {
+  using J = std::conditional_t<kType == 0, Most, Sum>;
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < blocks; i += kThreads)
+    acc = J::join(acc, partial[i]);
+  acc = block_join<J>(acc);
+  if (threadIdx.x == 0) {
+    const float norm = static_cast<float>(kType == 2 ? sqrt(acc) : acc);
+    const float c = max_norm / (norm + 1e-6f);
+    out[0] = norm;
+    out[1] = c > 1.f ? 1.f : c;  // NaN stays
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void grad_scale_kernel(
+    const GradTable t, const float* __restrict__ factor) {
+  constexpr int V = kVec<T>;
+  constexpr int kAhead = 4;
+  const float c = *factor;
+  if (c == 1.f) return;
+  const int chunks = t.first[t.count];
+  for (int b = blockIdx.x; b < chunks; b += gridDim.x) {
+    const int i = tensor_of(t, b);
+    const int64_t begin = static_cast<int64_t>(b - t.first[i]) * kGradChunk;
+    T* p = static_cast<T*>(t.ptr[i]) + begin;
+    const int len = static_cast<int>(min(kGradChunk, t.n[i] - begin));
+    const int full = len / V;
+    int k = threadIdx.x;
+    for (; k + (kAhead - 1) * kThreads < full; k += kAhead * kThreads) {
+      u32x4 r[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) r[a] = load16(p + (k + a * kThreads) * V);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        float f[V];
+        unpack<T>(r[a], f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] *= c;
+        store16(p + (k + a * kThreads) * V, pack<T>(f));
+      }
+    }
+    for (; k < full; k += kThreads) {
+      float f[V];
+      unpack<T>(load16(p + k * V), f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] *= c;
+      store16(p + k * V, pack<T>(f));
+    }
+    for (int j = full * V + threadIdx.x; j < len; j += kThreads)
+      p[j] = static_cast<T>(static_cast<float>(p[j]) * c);
+  }
+}
+
+template <int kType>
+void partial_of(const GradTable& t, int dtype, double* partial,
+                hipStream_t stream) {
+  auto* k = dtype == kFloat  ? grad_partial_kernel<float, kType>
+            : dtype == kHalf ? grad_partial_kernel<_Float16, kType>
+                             : grad_partial_kernel<__bf16, kType>;
+  hipLaunchKernelGGL(k, dim3(grad_norm_blocks(t)), dim3(kThreads), 0, stream, t,
+                     partial);
+}
+
+}  // namespace
+
+int grad_norm_blocks(const GradTable& t) {
+  return std::min(kMaxBlocks, t.first[t.count]);
+}
+
+void launch_grad_partial(const GradTable& t, int dtype, int type,
+                         double* partial, hipStream_t stream) {
+  if (type == 2) partial_of<2>(t, dtype, partial, stream);
+  if (type == 1) partial_of<1>(t, dtype, partial, stream);
+  if (type == 0) partial_of<0>(t, dtype, partial, stream);
+}
+
+void launch_grad_finish(const double* partial, int blocks, int type,
+                        float max_norm, float* out, hipStream_t stream) {
+  auto* k = type == 2   ? grad_finish_kernel<2>
+            : type == 1 ? grad_finish_kernel<1>
+                        : grad_finish_kernel<0>;
+  hipLaunchKernelGGL(k, dim3(1), dim3(kThreads), 0, stream, partial, blocks,
+                     max_norm, out);
+}
+
+void launch_grad_scale(const GradTable& t, int dtype, const float* factor,
+                       hipStream_t stream) {
+  auto* k = dtype == kFloat  ? grad_scale_kernel<float>
+            : dtype == kHalf ? grad_scale_kernel<_Float16>
+                             : grad_scale_kernel<__bf16>;
+  hipLaunchKernelGGL(k, dim3(std::min(kMaxBlocks, t.first[t.count])),
+                     dim3(kThreads), 0, stream, t, factor);
+}
+
+}  // namespace axon

@@ -106,6 +106,40 @@ void launch_swiglu_fwd(int dtype, const void* a, const void* g, void* z,
 void launch_swiglu_bwd(int dtype, const void* dz, const void* a, const void* g,
                        void* da, void* dg, int64_t numel, hipStream_t stream);
 
+// Embedding (embedding.hip): ids int32 or int64 [n], w [vocab, dim] with rows
+// wstride values apart, y/dy [n, dim] and dw [vocab, dim] contiguous.
+// Backward scratch: keys uint64[2n], part fp32[embed_part_floats(...)];
+// padding: the id without a gradient, or -1. Needs dim > 0 and n < 2^31;
+// forward needs n > 0.
+int64_t embed_part_floats(int64_t n, int64_t dim, int elem_size);
+void launch_embed_fwd(int dtype, bool ids64, const void* ids, const void* w,
+                      void* y, int64_t n, int64_t vocab, int64_t dim,
+                      int64_t wstride, float scale, hipStream_t stream);
+void launch_embed_bwd(int dtype, bool ids64, const void* ids, const void* dy,
+                      void* dw, uint64_t* keys, float* part, int64_t n,
+                      int64_t vocab, int64_t dim, int64_t padding, float scale,
+                      hipStream_t stream);
+
+// Cross entropy (cross_entropy.hip): row r of the logits starts at
+// (r / inner) * stride_outer + (r % inner) * stride_inner and is dense; dx is
+// [n, vocab] contiguous. reduction: 0 none (loss fp32[n]), 1 mean, 2 sum
+// (loss fp32[1]). kept fp32[2n] and factor fp32[1] (null in the backward pass
+// of reduction 0) go from forward to backward. gout: the loss's gradient, one
+// for each row (gstride 1) or one for all (0).
+int64_t ce_scratch_bytes(int64_t n, int64_t vocab);
+void launch_ce_fwd(int dtype, const void* x, int64_t inner,
+                   int64_t stride_outer, int64_t stride_inner,
+                   const int64_t* target, int64_t ignore, int64_t n,
+                   int64_t vocab, float eps, int reduction, void* scratch,
+                   float* kept, float* loss, float* factor,
+                   hipStream_t stream);
+void launch_ce_bwd(int dtype, const void* x, int64_t inner,
+                   int64_t stride_outer, int64_t stride_inner,
+                   const int64_t* target, int64_t ignore, int64_t n,
+                   int64_t vocab, float eps, const float* kept,
+                   const float* gout, int gstride, const float* factor,
+                   void* dx, hipStream_t stream);
+
 // EXPERIMENTAL flash-attention forward (flash_attn.hip, docs/FA_PLAN.md):
 // q/k/v/o are [B, H(Q|K), S, 128] contiguous bf16; lse fp32 [B, HQ, S]
 // (nullable). v0 correctness build, reachable only via tools/fa_probe.py.

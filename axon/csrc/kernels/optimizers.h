@@ -20,18 +20,21 @@ struct OptChunk {
   int64_t tidx;
 };
 
+// gscale: null, or a device scalar that every gradient is multiplied by (in
+// fp32, without a rounding of its own) before it is used: the clipping factor.
 void launch_fused_sgd(const OptChunk* chunks, int nchunks, int dtype, float lr,
                       float momentum, float dampening, float wd, bool nesterov,
-                      bool maximize, hipStream_t stream);
+                      bool maximize, const float* gscale, hipStream_t stream);
 
 void launch_fused_adam(const OptChunk* chunks, int nchunks, int dtype, float lr,
                        float beta1, float beta2, float eps, float wd, float bc1,
-                       float bc2_sqrt, bool adamw, hipStream_t stream);
+                       float bc2_sqrt, bool adamw, const float* gscale,
+                       hipStream_t stream);
 
 void launch_fused_lamb_phase1(const OptChunk* chunks, int nchunks, int dtype,
                               float beta1, float beta2, float eps, float wd,
                               float bc1, float bc2_sqrt, float* norms,
-                              hipStream_t stream);
+                              const float* gscale, hipStream_t stream);
 void launch_fused_lamb_phase2(const OptChunk* chunks, int nchunks, int dtype,
                               float lr, const float* norms, hipStream_t stream);
 

@@ -53,12 +53,17 @@ struct alignas(sizeof(T) * V) TVec {
 template <typename T>
 __global__ void sgd_kernel(const OptChunk* __restrict__ chunks, float lr,
                            float momentum, float dampening, float wd,
-                           int nesterov, int maximize) {
+                           int nesterov, int maximize,
+                           const float* __restrict__ gscale) {
   const OptChunk c = chunks[blockIdx.x];
   T* __restrict__ p = static_cast<T*>(c.p);
   const T* __restrict__ g = static_cast<const T*>(c.g);
   T* __restrict__ m = static_cast<T*>(c.m);
   constexpr int V = 8;
+  const float gs = gscale ? *gscale : 1.f;
+  // A choice, not a product with 1: without a factor the products and sums
+  // below contract as they do without this line.
+  auto scaled = [&](T gv) { return gscale ? f_of(gv) * gs : f_of(gv); };
   const bool vec = c.n % V == 0 &&
       (reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) |
        reinterpret_cast<uintptr_t>(m)) % (sizeof(T) * V) == 0;
@@ -82,7 +87,7 @@ __global__ void sgd_kernel(const OptChunk* __restrict__ chunks, float lr,
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         float pm = momentum != 0.f ? f_of(mm.v[k]) : 0.f;
-        float out = update(f_of(pp.v[k]), f_of(gg.v[k]), pm, &pm);
+        float out = update(f_of(pp.v[k]), scaled(gg.v[k]), pm, &pm);
         pp.v[k] = t_of<T>(out);
         if (momentum != 0.f) mm.v[k] = t_of<T>(pm);
       }
@@ -92,7 +97,7 @@ __global__ void sgd_kernel(const OptChunk* __restrict__ chunks, float lr,
   } else {
     for (int64_t i = threadIdx.x; i < c.n; i += kThreads) {
       float pm = momentum != 0.f ? f_of(m[i]) : 0.f;
-      float out = update(f_of(p[i]), f_of(g[i]), pm, &pm);
+      float out = update(f_of(p[i]), scaled(g[i]), pm, &pm);
       p[i] = t_of<T>(out);
       if (momentum != 0.f) m[i] = t_of<T>(pm);
     }
@@ -104,13 +109,18 @@ __global__ void sgd_kernel(const OptChunk* __restrict__ chunks, float lr,
 template <typename T>
 __global__ void adam_kernel(const OptChunk* __restrict__ chunks, float lr,
                             float beta1, float beta2, float eps, float wd,
-                            float bc1, float bc2_sqrt, int adamw) {
+                            float bc1, float bc2_sqrt, int adamw,
+                            const float* __restrict__ gscale) {
   const OptChunk c = chunks[blockIdx.x];
   T* __restrict__ p = static_cast<T*>(c.p);
   const T* __restrict__ g = static_cast<const T*>(c.g);
   T* __restrict__ m = static_cast<T*>(c.m);
   T* __restrict__ v = static_cast<T*>(c.v);
   constexpr int V = 8;
+  const float gs = gscale ? *gscale : 1.f;
+  // A choice, not a product with 1: without a factor the products and sums
+  // below contract as they do without this line.
+  auto scaled = [&](T gv) { return gscale ? f_of(gv) * gs : f_of(gv); };
   const bool vec = c.n % V == 0 &&
       (reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) |
        reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) %
@@ -137,7 +147,7 @@ __global__ void adam_kernel(const OptChunk* __restrict__ chunks, float lr,
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         float mf = f_of(mm.v[k]), vf = f_of(vv_.v[k]);
-        float out = update(f_of(pp.v[k]), f_of(gg.v[k]), &mf, &vf);
+        float out = update(f_of(pp.v[k]), scaled(gg.v[k]), &mf, &vf);
         pp.v[k] = t_of<T>(out);
         mm.v[k] = t_of<T>(mf);
         vv_.v[k] = t_of<T>(vf);
@@ -149,7 +159,7 @@ __global__ void adam_kernel(const OptChunk* __restrict__ chunks, float lr,
   } else {
     for (int64_t i = threadIdx.x; i < c.n; i += kThreads) {
       float mf = f_of(m[i]), vf = f_of(v[i]);
-      float out = update(f_of(p[i]), f_of(g[i]), &mf, &vf);
+      float out = update(f_of(p[i]), scaled(g[i]), &mf, &vf);
       p[i] = t_of<T>(out);
       m[i] = t_of<T>(mf);
       v[i] = t_of<T>(vf);
@@ -185,16 +195,21 @@ template <typename T>
 __global__ void lamb_phase1_kernel(const OptChunk* __restrict__ chunks,
                                    float beta1, float beta2, float eps,
                                    float wd, float bc1, float bc2_sqrt,
-                                   float* __restrict__ norms /* [ntensor][2] */) {
+                                   float* __restrict__ norms /* [ntensor][2] */,
+                                   const float* __restrict__ gscale) {
   const OptChunk c = chunks[blockIdx.x];
   T* __restrict__ p = static_cast<T*>(c.p);
   const T* __restrict__ g = static_cast<const T*>(c.g);
   T* __restrict__ m = static_cast<T*>(c.m);
   T* __restrict__ v = static_cast<T*>(c.v);
   float* __restrict__ u = static_cast<float*>(c.u);
+  const float gs = gscale ? *gscale : 1.f;
+  // A choice, not a product with 1: without a factor the products and sums
+  // below contract as they do without this line.
+  auto scaled = [&](T gv) { return gscale ? f_of(gv) * gs : f_of(gv); };
   float pn = 0.f, un = 0.f;
   for (int64_t i = threadIdx.x; i < c.n; i += kThreads) {
-    float pv = f_of(p[i]), gv = f_of(g[i]);
+    float pv = f_of(p[i]), gv = scaled(g[i]);
     float mf = beta1 * f_of(m[i]) + (1.f - beta1) * gv;
     float vf = beta2 * f_of(v[i]) + (1.f - beta2) * gv * gv;
     m[i] = t_of<T>(mf);
@@ -266,30 +281,31 @@ __global__ void lamb_phase2_kernel(const OptChunk* __restrict__ chunks, float lr
 
 void launch_fused_sgd(const OptChunk* chunks, int nchunks, int dtype, float lr,
                       float momentum, float dampening, float wd, bool nesterov,
-                      bool maximize, hipStream_t stream) {
+                      bool maximize, const float* gscale, hipStream_t stream) {
   if (nchunks <= 0) return;
   dim3 grid(nchunks), block(kThreads);
   DISPATCH(sgd_kernel, chunks, lr, momentum, dampening, wd, nesterov ? 1 : 0,
-           maximize ? 1 : 0);
+           maximize ? 1 : 0, gscale);
 }
 
 void launch_fused_adam(const OptChunk* chunks, int nchunks, int dtype, float lr,
                        float beta1, float beta2, float eps, float wd, float bc1,
-                       float bc2_sqrt, bool adamw, hipStream_t stream) {
+                       float bc2_sqrt, bool adamw, const float* gscale,
+                       hipStream_t stream) {
   if (nchunks <= 0) return;
   dim3 grid(nchunks), block(kThreads);
   DISPATCH(adam_kernel, chunks, lr, beta1, beta2, eps, wd, bc1, bc2_sqrt,
-           adamw ? 1 : 0);
+           adamw ? 1 : 0, gscale);
 }
 
 void launch_fused_lamb_phase1(const OptChunk* chunks, int nchunks, int dtype,
                               float beta1, float beta2, float eps, float wd,
                               float bc1, float bc2_sqrt, float* norms,
-                              hipStream_t stream) {
+                              const float* gscale, hipStream_t stream) {
   if (nchunks <= 0) return;
   dim3 grid(nchunks), block(kThreads);
   DISPATCH(lamb_phase1_kernel, chunks, beta1, beta2, eps, wd, bc1, bc2_sqrt,
-           norms);
+           norms, gscale);
 }
 
 void launch_fused_lamb_phase2(const OptChunk* chunks, int nchunks, int dtype,

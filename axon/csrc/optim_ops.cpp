@@ -92,9 +92,21 @@ hipStream_t cur_stream(const at::Tensor& t) {
       .stream();
 }
 
+// The clipping factor that the step multiplies the gradients by, or null.
+const float* scale_ptr(const c10::optional<at::Tensor>& t,
+                       const at::Tensor& like) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->device() == like.device() && t->scalar_type() == at::kFloat &&
+                  t->numel() == 1,
+              "fused optimizer: grad_scale must be one float on the "
+              "parameters' device");
+  return t->data_ptr<float>();
+}
+
 void fused_sgd(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                std::vector<at::Tensor> ms, double lr, double momentum,
-               double dampening, double wd, bool nesterov, bool maximize) {
+               double dampening, double wd, bool nesterov, bool maximize,
+               c10::optional<at::Tensor> grad_scale) {
   if (ps.empty()) return;
   auto plan = build_chunks(ps, gs, momentum != 0 ? ms : std::vector<at::Tensor>{},
                            {}, nullptr);
@@ -105,13 +117,15 @@ void fused_sgd(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
   launch_fused_sgd(reinterpret_cast<const OptChunk*>(plan.dev.data_ptr()),
                    plan.nchunks, dtype_code(ps[0]), static_cast<float>(lr),
                    static_cast<float>(momentum), static_cast<float>(dampening),
-                   static_cast<float>(wd), nesterov, maximize, cur_stream(ps[0]));
+                   static_cast<float>(wd), nesterov, maximize,
+                   scale_ptr(grad_scale, ps[0]), cur_stream(ps[0]));
 }
 
 void fused_adam(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                 std::vector<at::Tensor> ms, std::vector<at::Tensor> vs,
                 double lr, double beta1, double beta2, double eps, double wd,
-                int64_t step, bool adamw) {
+                int64_t step, bool adamw,
+                c10::optional<at::Tensor> grad_scale) {
   if (ps.empty()) return;
   auto plan = build_chunks(ps, gs, ms, vs, nullptr);
   float bc1 = 1.0f - std::pow(static_cast<float>(beta1), static_cast<float>(step));
@@ -121,13 +135,14 @@ void fused_adam(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                     plan.nchunks, dtype_code(ps[0]), static_cast<float>(lr),
                     static_cast<float>(beta1), static_cast<float>(beta2),
                     static_cast<float>(eps), static_cast<float>(wd), bc1,
-                    bc2_sqrt, adamw, cur_stream(ps[0]));
+                    bc2_sqrt, adamw, scale_ptr(grad_scale, ps[0]),
+                    cur_stream(ps[0]));
 }
 
 void fused_lamb(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                 std::vector<at::Tensor> ms, std::vector<at::Tensor> vs,
                 double lr, double beta1, double beta2, double eps, double wd,
-                int64_t step) {
+                int64_t step, c10::optional<at::Tensor> grad_scale) {
   if (ps.empty()) return;
   int64_t total = 0;
   for (auto& p : ps) total += p.numel();
@@ -144,7 +159,7 @@ void fused_lamb(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                            static_cast<float>(beta1), static_cast<float>(beta2),
                            static_cast<float>(eps), static_cast<float>(wd), bc1,
                            bc2_sqrt, static_cast<float*>(norms.data_ptr()),
-                           stream);
+                           scale_ptr(grad_scale, ps[0]), stream);
   launch_fused_lamb_phase2(descs, plan.nchunks, dtype_code(ps[0]),
                            static_cast<float>(lr),
                            static_cast<const float*>(norms.data_ptr()), stream);
@@ -157,16 +172,19 @@ void register_optim(pybind11::module_& m) {
         pybind11::arg("momentum_buffers"), pybind11::arg("lr"),
         pybind11::arg("momentum"), pybind11::arg("dampening"),
         pybind11::arg("weight_decay"), pybind11::arg("nesterov"),
-        pybind11::arg("maximize"));
+        pybind11::arg("maximize"),
+        pybind11::arg("grad_scale") = pybind11::none());
   m.def("fused_adam", &fused_adam, pybind11::arg("params"), pybind11::arg("grads"),
         pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"),
         pybind11::arg("lr"), pybind11::arg("beta1"), pybind11::arg("beta2"),
         pybind11::arg("eps"), pybind11::arg("weight_decay"), pybind11::arg("step"),
-        pybind11::arg("adamw"));
+        pybind11::arg("adamw"),
+        pybind11::arg("grad_scale") = pybind11::none());
   m.def("fused_lamb", &fused_lamb, pybind11::arg("params"), pybind11::arg("grads"),
         pybind11::arg("exp_avgs"), pybind11::arg("exp_avg_sqs"),
         pybind11::arg("lr"), pybind11::arg("beta1"), pybind11::arg("beta2"),
-        pybind11::arg("eps"), pybind11::arg("weight_decay"), pybind11::arg("step"));
+        pybind11::arg("eps"), pybind11::arg("weight_decay"), pybind11::arg("step"),
+        pybind11::arg("grad_scale") = pybind11::none());
 }
 
 }  // namespace axon

@@ -10,6 +10,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 
+from axon.ops.cross_entropy import cross_entropy
+from axon.ops.embedding import FusedEmbedding
 from axon.ops.layernorm import FusedLayerNorm
 import torch.nn.functional as F
 
@@ -80,7 +82,7 @@ class BertForPreTraining(nn.Module):
     def __init__(self, cfg: BertConfig):
         super().__init__()
         self.cfg = cfg
-        self.tok = nn.Embedding(cfg.vocab_size, cfg.hidden)
+        self.tok = FusedEmbedding(cfg.vocab_size, cfg.hidden)
         self.pos = nn.Embedding(cfg.max_seq, cfg.hidden)
         self.typ = nn.Embedding(cfg.type_vocab, cfg.hidden)
         self.ln_emb = FusedLayerNorm(cfg.hidden)
@@ -113,6 +115,5 @@ class BertForPreTraining(nn.Module):
 
     def mlm_loss(self, input_ids, labels, **kw):
         """labels = -100 where not masked (standard MLM convention)."""
-        logits = self.forward(input_ids, **kw)
-        return F.cross_entropy(logits.float().view(-1, self.cfg.vocab_size),
-                               labels.view(-1), ignore_index=-100)
+        return cross_entropy(self.forward(input_ids, **kw), labels,
+                             ignore_index=-100)

@@ -13,6 +13,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from axon.ops.cross_entropy import cross_entropy
+from axon.ops.embedding import FusedEmbedding
 from axon.ops.rmsnorm import FusedRMSNorm
 from axon.ops.rotary import rope, swiglu
 
@@ -118,7 +120,7 @@ class LlamaForCausalLM(nn.Module):
     def __init__(self, cfg: LlamaConfig):
         super().__init__()
         self.cfg = cfg
-        self.embed = nn.Embedding(cfg.vocab_size, cfg.dim)
+        self.embed = FusedEmbedding(cfg.vocab_size, cfg.dim)
         self.blocks = nn.ModuleList(LlamaBlock(cfg) for _ in range(cfg.layers))
         self.norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.lm_head = nn.Linear(cfg.dim, cfg.vocab_size, bias=False)
@@ -155,9 +157,11 @@ class LlamaForCausalLM(nn.Module):
     def lm_loss(self, input_ids):
         """Next-token loss on the sequence itself (synthetic pretrain)."""
         logits = self.forward(input_ids)
-        return F.cross_entropy(
-            logits[:, :-1].float().reshape(-1, self.cfg.vocab_size),
-            input_ids[:, 1:].reshape(-1))
+        # Each position's label is the next token and the last one has none:
+        # the loss reads the logits whole, and its gradient is written whole
+        # (a slice's gradient would be copied into zeros once more).
+        return cross_entropy(logits, F.pad(input_ids[:, 1:], (0, 1),
+                                           value=-100))
 
     @torch.no_grad()
     def generate(self, input_ids, max_new_tokens, temperature=0.0,

@@ -8,4 +8,5 @@ PyTorch. On CPU tensors the step falls back to the identical formulas in
 Python (also the numerics oracle for the GPU kernels: tests/test_gpu.py).
 On a GPU box the HIP path is mandatory — a missing extension raises.
 """
+from axon.optim.clip import clip_grad_norm_, grad_norm  # noqa: F401
 from axon.optim.fused import FusedAdam, FusedAdamW, FusedLAMB, FusedSGD  # noqa: F401

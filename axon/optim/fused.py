@@ -4,6 +4,8 @@ import math
 import torch
 from torch.optim import Optimizer
 
+from axon.optim.clip import _checked_max, norm_and_factor
+
 
 def _like_param(p, t):
     """The fused kernels walk flat storage, so grad/state must share the
@@ -27,11 +29,51 @@ def _grouped(params_with_grad):
     return groups.values()
 
 
-class FusedSGD(Optimizer):
+class _Clipping(Optimizer):
+    """max_grad_norm: step() first takes the norm over the gradients of ALL
+    groups, and the fused kernels multiply each gradient by the clipping
+    factor as they read it (p.grad itself stays as it is). grad_norm is the
+    last step's norm, a 0-dim tensor. Not part of the state dict, which stays
+    the stock optimizers'; copies and pickles keep it."""
+    max_grad_norm = None
+    grad_norm = None
+
+    def _init_clipping(self, max_grad_norm):
+        if max_grad_norm is not None:
+            self.max_grad_norm = _checked_max(max_grad_norm)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
+
+    def _clip_factor(self):
+        """The factor for this step, or None."""
+        if self.max_grad_norm is None:
+            return None
+        grads = [p.grad for group in self.param_groups
+                 for p in group["params"] if p.grad is not None]
+        if not grads:
+            return None
+        self.grad_norm, factor = norm_and_factor(grads, self.max_grad_norm)
+        return factor.float()
+
+
+def _factor_for(factor, p):
+    return None if factor is None else factor.to(p.device)
+
+
+def _clipped(gs, factor):
+    """The gradients as the CPU formulas take them."""
+    if factor is None:
+        return gs
+    return [g.float() * _factor_for(factor, g) for g in gs]
+
+
+class FusedSGD(_Clipping):
     """torch.optim.SGD semantics, one HIP kernel launch per group."""
 
     def __init__(self, params, lr=0.1, momentum=0.0, dampening=0.0,
-                 weight_decay=0.0, nesterov=False, maximize=False):
+                 weight_decay=0.0, nesterov=False, maximize=False,
+                 max_grad_norm=None):
         if nesterov and (momentum <= 0 or dampening != 0):
             raise ValueError("nesterov requires momentum > 0, dampening 0")
         if dampening != 0 and 0 < momentum < 1e-8:
@@ -45,6 +87,7 @@ class FusedSGD(Optimizer):
                                       dampening=dampening,
                                       weight_decay=weight_decay,
                                       nesterov=nesterov, maximize=maximize))
+        self._init_clipping(max_grad_norm)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -54,6 +97,7 @@ class FusedSGD(Optimizer):
                 loss = closure()
         from axon import _core
 
+        factor = self._clip_factor()
         for group in self.param_groups:
             work = []
             mu = group["momentum"]
@@ -74,6 +118,8 @@ class FusedSGD(Optimizer):
                         # mu*m + (1-damp)*d equal d on the first step.
                         g0 = _like_param(p, p.grad)
                         d0 = (-g0 if group["maximize"] else g0).float()
+                        if factor is not None:
+                            d0 = d0 * factor.to(d0.device)
                         if group["weight_decay"] != 0:
                             d0 = d0 + group["weight_decay"] * p.detach().float()
                         st["momentum_buffer"] = \
@@ -90,9 +136,10 @@ class FusedSGD(Optimizer):
                     _core.fused_sgd([p.data for p in ps], gs, ms, group["lr"],
                                     mu, group["dampening"],
                                     group["weight_decay"], group["nesterov"],
-                                    group["maximize"])
+                                    group["maximize"],
+                                    _factor_for(factor, ps[0]))
                 else:
-                    self._step_cpu(ps, gs, ms, group)
+                    self._step_cpu(ps, _clipped(gs, factor), ms, group)
         return loss
 
     @staticmethod
@@ -110,13 +157,14 @@ class FusedSGD(Optimizer):
             p.data.copy_(p.float() - group["lr"] * d)
 
 
-class _FusedAdamBase(Optimizer):
+class _FusedAdamBase(_Clipping):
     _adamw = False
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
-                 weight_decay=0.0):
+                 weight_decay=0.0, max_grad_norm=None):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps,
                                       weight_decay=weight_decay))
+        self._init_clipping(max_grad_norm)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -126,6 +174,7 @@ class _FusedAdamBase(Optimizer):
                 loss = closure()
         from axon import _core
 
+        factor = self._clip_factor()
         for group in self.param_groups:
             work = []
             for p in group["params"]:
@@ -157,10 +206,10 @@ class _FusedAdamBase(Optimizer):
                         _core.fused_adam([p.data for p in ps], gs, ms, vs,
                                          group["lr"], b1, b2, group["eps"],
                                          group["weight_decay"], step_count,
-                                         self._adamw)
+                                         self._adamw, _factor_for(factor, ps[0]))
                     else:
-                        self._step_cpu(ps, gs, ms, vs, group, step_count,
-                                       self._adamw)
+                        self._step_cpu(ps, _clipped(gs, factor), ms, vs,
+                                       group, step_count, self._adamw)
         return loss
 
     @staticmethod
@@ -195,7 +244,7 @@ class FusedAdamW(_FusedAdamBase):
     _adamw = True
 
 
-class FusedLAMB(Optimizer):
+class FusedLAMB(_Clipping):
     """LAMB (You et al., Large Batch Optimization for Deep Learning):
     Adam-style update direction with decoupled weight decay, scaled per
     tensor by trust ratio ||p|| / ||update||. Two fused HIP phases: phase 1
@@ -204,9 +253,10 @@ class FusedLAMB(Optimizer):
     uses this."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-6,
-                 weight_decay=0.0):
+                 weight_decay=0.0, max_grad_norm=None):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps,
                                       weight_decay=weight_decay))
+        self._init_clipping(max_grad_norm)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -216,6 +266,7 @@ class FusedLAMB(Optimizer):
                 loss = closure()
         from axon import _core
 
+        factor = self._clip_factor()
         for group in self.param_groups:
             work = []
             for p in group["params"]:
@@ -244,9 +295,11 @@ class FusedLAMB(Optimizer):
                     if ps[0].is_cuda:
                         _core.fused_lamb([p.data for p in ps], gs, ms, vs,
                                          group["lr"], b1, b2, group["eps"],
-                                         group["weight_decay"], step_count)
+                                         group["weight_decay"], step_count,
+                                         _factor_for(factor, ps[0]))
                     else:
-                        self._step_cpu(ps, gs, ms, vs, group, step_count)
+                        self._step_cpu(ps, _clipped(gs, factor), ms, vs,
+                                       group, step_count)
         return loss
 
     @staticmethod
