@@ -9,7 +9,13 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+
 #include <algorithm>
+#include <mutex>
 #include <unordered_map>
 
 #include "kernels/grad_norm.h"
@@ -38,45 +44,28 @@ void check_launch() {
               hipGetErrorString(e));
 }
 
+// A gradient that must not be differentiated again, under create_graph.
+at::Tensor once(at::Tensor grad, const char* what) {
+  if (!at::GradMode::is_enabled()) return grad;
+  auto f = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + ": the gradient is not differentiable again", 1);
+  return (*f)({std::move(grad)})[0];
+}
+
+// Forward-mode tangents would be lost without a word.
+void check_no_tangent(const at::Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what,
+                              ": no forward-mode derivative");
+}
+
+// The nodes below are written against torch's graph itself: a Python
+// autograd.Function costs about 20 us for each pass through it, more than
+// the kernels of a small batch.
+
 // ------------------------------------------------------------- embedding
-
-void check_ids(const at::Tensor& ids, const at::Tensor& other) {
-  TORCH_CHECK(ids.is_cuda() && ids.device() == other.device(),
-              "embedding: ids and weight must be on the same GPU");
-  TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt,
-              "embedding: ids must be int32 or int64");
-  TORCH_CHECK(ids.is_contiguous() && ids.numel() < (int64_t{1} << 31),
-              "embedding: ids must be contiguous, fewer than 2^31");
-}
-
-at::Tensor embed_fwd(const at::Tensor& ids, const at::Tensor& w, double scale) {
-  check_ids(ids, w);
-  TORCH_CHECK(w.dim() == 2 && float_type(w) &&
-                  (w.size(1) <= 1 || w.stride(1) == 1) &&
-                  w.size(1) < (int64_t{1} << 22),
-              "embedding: weight must be [V, D] float/half/bfloat16 with "
-              "dense rows of fewer than 2^22 values");
-  auto shape = ids.sizes().vec();
-  shape.push_back(w.size(1));
-  const Guard guard(w.device());
-  at::Tensor y = at::empty(shape, w.options());
-  if (y.numel() == 0) return y;
-  launch_embed_fwd(code_of(w), ids.scalar_type() == at::kLong, ids.data_ptr(),
-                   w.data_ptr(), y.data_ptr(), ids.numel(), w.size(0),
-                   w.size(1), w.stride(0), static_cast<float>(scale),
-                   stream_of(w));
-  check_launch();
-  return y;
-}
 
 at::Tensor embed_bwd(const at::Tensor& ids, const at::Tensor& dy_in,
                      int64_t vocab, int64_t padding, double scale) {
-  check_ids(ids, dy_in);
-  TORCH_CHECK(float_type(dy_in) && dy_in.dim() >= 1 &&
-                  dy_in.sizes().slice(0, dy_in.dim() - 1) == ids.sizes(),
-              "embedding: gradient must be ids' shape x D");
-  TORCH_CHECK(vocab >= 0 && vocab < (int64_t{1} << 31),
-              "embedding: fewer than 2^31 rows");
   const Guard guard(dy_in.device());
   const at::Tensor dy = dy_in.contiguous();
   const int64_t n = ids.numel(), dim = dy.size(-1);
@@ -95,6 +84,89 @@ at::Tensor embed_bwd(const at::Tensor& ids, const at::Tensor& dy_in,
   return dw;
 }
 
+struct EmbeddingBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable ids;
+  int64_t vocab = 0, padding = -1;
+  double scale = 1.0;
+
+  torch::autograd::variable_list apply(
+      torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor i = ids.unpack(shared_from_this());
+    if (!grads[0].defined()) return {at::Tensor()};
+    at::Tensor dw;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      dw = embed_bwd(i, grads[0], vocab, padding, scale);
+    }
+    return {once(dw, "embedding")};
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ids.reset_data();
+  }
+  std::string name() const override { return "AxonEmbeddingBackward"; }
+};
+
+at::Tensor embedding(const at::Tensor& ids_in, const at::Tensor& weight_in,
+                     double scale, c10::optional<int64_t> padding_idx) {
+  TORCH_CHECK_VALUE(weight_in.dim() == 2, "embedding: weight must be [V, D], "
+                    "got ", weight_in.sizes());
+  TORCH_CHECK_TYPE(ids_in.scalar_type() == at::kLong ||
+                       ids_in.scalar_type() == at::kInt,
+                   "embedding: ids must be int32 or int64, got ",
+                   ids_in.scalar_type());
+  const int64_t vocab = weight_in.size(0), dim = weight_in.size(1);
+  int64_t padding = -1;
+  if (padding_idx.has_value()) {
+    TORCH_CHECK_VALUE(*padding_idx >= -vocab && *padding_idx < vocab,
+                      "embedding: padding_idx ", *padding_idx, " outside the ",
+                      vocab, " rows");
+    padding = *padding_idx < 0 ? *padding_idx + vocab : *padding_idx;
+  }
+  TORCH_CHECK_VALUE(weight_in.is_cuda() && ids_in.device() == weight_in.device(),
+                    "embedding: ids on ", ids_in.device(), ", weight on ",
+                    weight_in.device());
+  TORCH_CHECK_TYPE(float_type(weight_in),
+                   "embedding: weight must be float, half or bfloat16");
+  TORCH_CHECK_VALUE(vocab < (int64_t{1} << 31) && dim < (int64_t{1} << 22) &&
+                        ids_in.numel() < (int64_t{1} << 31),
+                    "embedding: fewer than 2^31 rows and ids, and rows of "
+                    "fewer than 2^22 values");
+  check_no_tangent(weight_in, "embedding");
+  const Guard guard(weight_in.device());
+  const at::Tensor weight = dim > 1 && weight_in.stride(1) != 1
+                                ? weight_in.contiguous()
+                                : weight_in;
+  const at::Tensor ids = ids_in.contiguous();
+  std::shared_ptr<EmbeddingBackward> node;
+  if (torch::autograd::compute_requires_grad(weight)) {
+    node = std::shared_ptr<EmbeddingBackward>(new EmbeddingBackward(),
+                                              torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(weight));
+    node->ids = torch::autograd::SavedVariable(ids, false);
+    node->vocab = vocab;
+    node->padding = padding;
+    node->scale = scale;
+  }
+  at::Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto shape = ids.sizes().vec();
+    shape.push_back(dim);
+    y = at::empty(shape, weight.options());
+  }
+  if (y.numel()) {
+    launch_embed_fwd(code_of(weight), ids.scalar_type() == at::kLong,
+                     ids.data_ptr(), weight.data_ptr(), y.data_ptr(),
+                     ids.numel(), vocab, dim, weight.stride(0),
+                     static_cast<float>(scale), stream_of(weight));
+    check_launch();
+  }
+  if (node) torch::autograd::set_history(y, node);
+  return y;
+}
+
 // --------------------------------------------------------- cross entropy
 
 struct LogitRows {
@@ -104,70 +176,135 @@ struct LogitRows {
 // Logits [V], [N, V] or [B, S, V] with a dense last dimension; the others may
 // have any strides.
 LogitRows logit_rows(const at::Tensor& x, const at::Tensor& target) {
-  TORCH_CHECK(x.is_cuda() && target.is_cuda() && x.device() == target.device(),
-              "cross_entropy: logits and target must be on the same GPU");
-  TORCH_CHECK(float_type(x) && x.dim() >= 1 && x.dim() <= 3 &&
-                  x.size(-1) > 0 && (x.size(-1) == 1 || x.stride(-1) == 1),
-              "cross_entropy: logits must be [V], [N, V] or [B, S, V] "
-              "float/half/bfloat16 with a dense last dimension");
-  TORCH_CHECK(target.scalar_type() == at::kLong && target.is_contiguous() &&
-                  target.sizes() == x.sizes().slice(0, x.dim() - 1),
-              "cross_entropy: target must be contiguous int64 of the logits' "
-              "shape without the last dimension");
   LogitRows r;
   r.vocab = x.size(-1);
   r.n = target.numel();
   r.inner = x.dim() == 1 ? 1 : std::max<int64_t>(1, x.size(-2));
   r.stride_inner = x.dim() == 1 ? 0 : x.stride(-2);
   r.stride_outer = x.dim() == 3 ? x.stride(0) : 0;
-  TORCH_CHECK(r.n < (int64_t{1} << 31) / 4, "cross_entropy: too many rows");
   return r;
 }
 
-// Returns (loss, kept, factor): a 0-dim loss, or one of target's shape for
-// reduction 0; what the backward pass takes.
-std::vector<at::Tensor> ce_fwd(const at::Tensor& x, const at::Tensor& target,
-                               int64_t ignore, double eps, int64_t reduction) {
-  const LogitRows r = logit_rows(x, target);
-  TORCH_CHECK(reduction >= 0 && reduction <= 2, "cross_entropy: reduction");
-  const Guard guard(x.device());
-  const auto fopt = x.options().dtype(at::kFloat);
-  at::Tensor kept = at::empty({2 * r.n}, fopt);
-  at::Tensor factor = at::empty({1}, fopt);
-  at::Tensor loss = reduction == 0 ? at::empty(target.sizes(), fopt)
-                                   : at::empty({}, fopt);
-  at::Tensor scratch = at::empty({ce_scratch_bytes(r.n, r.vocab)},
-                                 x.options().dtype(at::kByte));
-  launch_ce_fwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
-                r.stride_inner, target.data_ptr<int64_t>(), ignore, r.n,
-                r.vocab, static_cast<float>(eps), static_cast<int>(reduction),
-                scratch.data_ptr(), kept.data_ptr<float>(),
-                loss.data_ptr<float>(), factor.data_ptr<float>(),
-                stream_of(x));
-  check_launch();
-  return {loss, kept, factor};
-}
+struct CrossEntropyBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable logits, target;
+  at::Tensor kept, factor;  // of this file alone
+  int64_t ignore = 0;
+  double eps = 0.0;
+  int reduction = 1;
 
-at::Tensor ce_bwd(const at::Tensor& x, const at::Tensor& target,
-                  int64_t ignore, double eps, int64_t reduction,
-                  const at::Tensor& kept, const at::Tensor& factor,
-                  const at::Tensor& gout_in) {
-  const LogitRows r = logit_rows(x, target);
-  TORCH_CHECK(gout_in.is_cuda() && gout_in.scalar_type() == at::kFloat &&
-                  gout_in.numel() == (reduction == 0 ? r.n : 1),
-              "cross_entropy: the loss's gradient");
-  const Guard guard(x.device());
-  const at::Tensor gout = gout_in.contiguous();
-  at::Tensor dx = at::empty(x.sizes(), x.options());
-  if (r.n == 0) return dx;
-  launch_ce_bwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
-                r.stride_inner, target.data_ptr<int64_t>(), ignore, r.n,
-                r.vocab, static_cast<float>(eps), kept.data_ptr<float>(),
-                gout.data_ptr<float>(), reduction == 0 ? 1 : 0,
-                reduction == 0 ? nullptr : factor.data_ptr<float>(),
-                dx.data_ptr(), stream_of(x));
-  check_launch();
-  return dx;
+  torch::autograd::variable_list apply(
+      torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor x = logits.unpack(), t = target.unpack();
+    if (!grads[0].defined()) return {at::Tensor()};
+    at::Tensor dx;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const LogitRows r = logit_rows(x, t);
+      const Guard guard(x.device());
+      const at::Tensor g = grads[0].contiguous();
+      TORCH_CHECK(g.is_cuda() && g.scalar_type() == at::kFloat &&
+                      g.numel() == (reduction == 0 ? r.n : 1),
+                  "cross_entropy: the loss's gradient");
+      dx = at::empty(x.sizes(), x.options());
+      if (r.n > 0) {
+        launch_ce_bwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
+                      r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n,
+                      r.vocab, static_cast<float>(eps),
+                      kept.data_ptr<float>(), g.data_ptr<float>(),
+                      reduction == 0 ? 1 : 0,
+                      reduction == 0 ? nullptr : factor.data_ptr<float>(),
+                      dx.data_ptr(), stream_of(x));
+        check_launch();
+      }
+    }
+    return {once(dx, "cross_entropy")};
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    logits.reset_data();
+    target.reset_data();
+    kept.reset();
+    factor.reset();
+  }
+  std::string name() const override { return "AxonCrossEntropyBackward"; }
+};
+
+at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
+                         int64_t ignore, double eps,
+                         const std::string& reduction_name) {
+  const int reduction = reduction_name == "none"   ? 0
+                        : reduction_name == "mean" ? 1
+                        : reduction_name == "sum"  ? 2
+                                                   : -1;
+  TORCH_CHECK_VALUE(reduction >= 0, "cross_entropy: reduction '",
+                    reduction_name, "', expected 'none', 'mean' or 'sum'");
+  TORCH_CHECK_VALUE(eps >= 0.0 && eps <= 1.0,
+                    "cross_entropy: label_smoothing outside [0, 1]: ", eps);
+  TORCH_CHECK_TYPE(target.scalar_type() == at::kLong ||
+                       target.scalar_type() == at::kInt,
+                   "cross_entropy: target must hold class numbers (int32 or "
+                   "int64), got ", target.scalar_type());
+  TORCH_CHECK_VALUE(
+      logits.dim() >= 1 && logits.size(-1) > 0 &&
+          target.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+      "cross_entropy: logits ", logits.sizes(), " and target ",
+      target.sizes(), ": one label for each row of classes");
+  TORCH_CHECK_VALUE(logits.is_cuda() && target.device() == logits.device(),
+                    "cross_entropy: target on ", target.device(),
+                    ", logits on ", logits.device());
+  TORCH_CHECK_TYPE(float_type(logits),
+                   "cross_entropy: logits must be float, half or bfloat16");
+  // The partial sums of more rows would take a third launch.
+  TORCH_CHECK_VALUE(target.numel() < (int64_t{1} << 28),
+                    "cross_entropy: too many rows");
+  check_no_tangent(logits, "cross_entropy");
+  const Guard guard(logits.device());
+  // With the caller's autograd: the gradient goes back through these.
+  at::Tensor x = logits, t = target;
+  if (x.size(-1) > 1 && x.stride(-1) != 1) x = x.contiguous();
+  if (x.dim() > 3) {
+    x = x.flatten(0, -3);
+    t = t.flatten(0, -2);
+  }
+  if (t.scalar_type() != at::kLong) t = t.to(at::kLong);
+  t = t.contiguous();
+  const LogitRows r = logit_rows(x, t);
+  std::shared_ptr<CrossEntropyBackward> node;
+  if (torch::autograd::compute_requires_grad(x)) {
+    node = std::shared_ptr<CrossEntropyBackward>(new CrossEntropyBackward(),
+                                                 torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->logits = torch::autograd::SavedVariable(x, false);
+    node->target = torch::autograd::SavedVariable(t, false);
+    node->ignore = ignore;
+    node->eps = eps;
+    node->reduction = reduction;
+  }
+  at::Tensor loss;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto fopt = x.options().dtype(at::kFloat);
+    // The loss, which its user may change in place, is memory of its own.
+    loss = reduction == 0 ? at::empty(target.sizes(), fopt)
+                          : at::empty({}, fopt);
+    at::Tensor kept = at::empty({2 * r.n + 1}, fopt);
+    at::Tensor factor = kept.narrow(0, 2 * r.n, 1);
+    at::Tensor scratch = at::empty({ce_scratch_bytes(r.n, r.vocab)},
+                                   x.options().dtype(at::kByte));
+    launch_ce_fwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
+                  r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n, r.vocab,
+                  static_cast<float>(eps), reduction, scratch.data_ptr(),
+                  kept.data_ptr<float>(), loss.data_ptr<float>(),
+                  factor.data_ptr<float>(), stream_of(x));
+    check_launch();
+    if (node) {
+      node->kept = kept;
+      node->factor = factor;
+    }
+  }
+  if (node) torch::autograd::set_history(loss, node);
+  return loss;
 }
 
 // ---------------------------------------------------------- gradient norm
@@ -317,17 +454,11 @@ void grad_scale_(const std::vector<at::Tensor>& ts, const at::Tensor& factor) {
 }  // namespace
 
 void register_lm(pybind11::module_& m) {
-  m.def("embed_fwd", &embed_fwd, py::arg("ids"), py::arg("weight"),
-        py::arg("scale"));
-  m.def("embed_bwd", &embed_bwd, py::arg("ids"), py::arg("dy"),
-        py::arg("vocab"), py::arg("padding"), py::arg("scale"));
-  m.def("ce_fwd", &ce_fwd, py::arg("logits"), py::arg("target"),
+  m.def("embedding", &embedding, py::arg("ids"), py::arg("weight"),
+        py::arg("scale"), py::arg("padding_idx"));
+  m.def("cross_entropy", &cross_entropy, py::arg("logits"), py::arg("target"),
         py::arg("ignore_index"), py::arg("label_smoothing"),
         py::arg("reduction"));
-  m.def("ce_bwd", &ce_bwd, py::arg("logits"), py::arg("target"),
-        py::arg("ignore_index"), py::arg("label_smoothing"),
-        py::arg("reduction"), py::arg("kept"), py::arg("factor"),
-        py::arg("grad_loss"));
   m.def("grad_norm", &grad_norm, py::arg("tensors"), py::arg("type"),
         py::arg("max_norm"));
   m.def("grad_scale_", &grad_scale_, py::arg("tensors"), py::arg("factor"));

@@ -4,31 +4,8 @@ gradient; no fp32 copy of them and no softmax is stored. Eager fallback off
 the GPU."""
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 _SUPPORTED = (torch.float32, torch.float16, torch.bfloat16)
-_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-
-
-class _CrossEntropyFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, target, ignore_index, smoothing, reduction):
-        from axon import _core
-
-        loss, kept, factor = _core.ce_fwd(logits, target, ignore_index,
-                                          smoothing, reduction)
-        ctx.save_for_backward(logits, target, kept, factor)
-        ctx.args = (ignore_index, smoothing, reduction)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss):
-        from axon import _core
-
-        logits, target, kept, factor = ctx.saved_tensors
-        return (_core.ce_bwd(logits, target, *ctx.args, kept, factor, dloss),
-                None, None, None, None)
 
 
 def cross_entropy(logits, target, ignore_index=-100, label_smoothing=0.0,
@@ -45,7 +22,12 @@ def cross_entropy(logits, target, ignore_index=-100, label_smoothing=0.0,
     and its row's gradient NaN (a check would wait for the GPU); on the CPU it
     raises IndexError. The gradient is not differentiable again.
     """
-    if reduction not in _REDUCTIONS:
+    if logits.is_cuda and logits.dtype in _SUPPORTED:
+        from axon import _core
+
+        return _core.cross_entropy(logits, target, ignore_index,
+                                   label_smoothing, reduction)
+    if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"cross_entropy: reduction {reduction!r}, expected "
                          "'none', 'mean' or 'sum'")
     if not 0.0 <= label_smoothing <= 1.0:
@@ -54,30 +36,16 @@ def cross_entropy(logits, target, ignore_index=-100, label_smoothing=0.0,
     if target.dtype not in (torch.int32, torch.int64):
         raise TypeError("cross_entropy: target must hold class numbers "
                         f"(int32 or int64), got {target.dtype}")
-    if logits.dim() < 1 or target.shape != logits.shape[:-1]:
-        raise ValueError(f"cross_entropy: logits {tuple(logits.shape)} need a "
-                         f"target of {tuple(logits.shape[:-1])}, got "
-                         f"{tuple(target.shape)}")
-    if logits.size(-1) == 0:
-        raise ValueError("cross_entropy: no classes")
-    target = target.long()
-    if logits.is_cuda and logits.dtype in _SUPPORTED:
-        if target.device != logits.device:
-            raise ValueError(f"cross_entropy: target on {target.device}, "
-                             f"logits on {logits.device}")
-        x, t = logits, target.contiguous()
-        if x.size(-1) > 1 and x.stride(-1) != 1:
-            x = x.contiguous()
-        if x.dim() > 3:
-            x, t = x.flatten(0, -3), t.flatten(0, -2)
-        loss = _CrossEntropyFunc.apply(x, t, ignore_index,
-                                       float(label_smoothing),
-                                       _REDUCTIONS[reduction])
-        return loss.view(target.shape) if reduction == "none" else loss
+    if (logits.dim() < 1 or logits.size(-1) == 0 or
+            target.shape != logits.shape[:-1]):
+        raise ValueError(f"cross_entropy: logits {tuple(logits.shape)} and "
+                         f"target {tuple(target.shape)}: one label for each "
+                         "row of classes")
     if logits.dtype in (torch.float16, torch.bfloat16):
         logits = logits.float()
     loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)),
-                           target.reshape(-1), ignore_index=ignore_index,
+                           target.reshape(-1).long(),
+                           ignore_index=ignore_index,
                            label_smoothing=label_smoothing,
                            reduction=reduction)
     return loss.view(target.shape) if reduction == "none" else loss

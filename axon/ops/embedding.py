@@ -1,34 +1,12 @@
 """Embedding lookup with scaling (csrc/kernels/embedding.hip): one pass over
 the named rows forward; backward sorts the tokens by id and sums each id's
-rows in order, so the gradient has the same bits each time (ATen's adds with
-atomics, or sorts with a library). Eager fallback off the GPU."""
+rows in order, so the gradient has the same bits each time. Eager fallback
+off the GPU."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 _SUPPORTED = (torch.float32, torch.float16, torch.bfloat16)
-
-
-class _EmbeddingFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx):
-        from axon import _core
-
-        ctx.save_for_backward(ids)
-        ctx.vocab = weight.size(0)
-        ctx.scale = scale
-        ctx.padding = -1 if padding_idx is None else padding_idx
-        return _core.embed_fwd(ids, weight, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        from axon import _core
-
-        (ids,) = ctx.saved_tensors
-        return (None, _core.embed_bwd(ids, dy, ctx.vocab, ctx.padding,
-                                      ctx.scale), None, None)
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None):
@@ -42,25 +20,20 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     check would wait for the GPU); on the CPU it raises IndexError. The
     gradient is not differentiable again.
     """
+    if weight.is_cuda and weight.dtype in _SUPPORTED:
+        from axon import _core
+
+        return _core.embedding(ids, weight, scale, padding_idx)
     if weight.dim() != 2:
         raise ValueError("embedding: weight must be [V, D], got "
                          f"{tuple(weight.shape)}")
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError("embedding: ids must be int32 or int64, got "
                         f"{ids.dtype}")
-    if padding_idx is not None:
-        if not -weight.size(0) <= padding_idx < weight.size(0):
-            raise ValueError(f"embedding: padding_idx {padding_idx} outside "
-                             f"the {weight.size(0)} rows")
-        padding_idx %= weight.size(0)
-    if weight.is_cuda and weight.dtype in _SUPPORTED:
-        if ids.device != weight.device:
-            raise ValueError(f"embedding: ids on {ids.device}, weight on "
-                             f"{weight.device}")
-        if weight.size(1) > 1 and weight.stride(1) != 1:
-            weight = weight.contiguous()
-        return _EmbeddingFunc.apply(ids.contiguous(), weight, float(scale),
-                                    padding_idx)
+    if padding_idx is not None and not (
+            -weight.size(0) <= padding_idx < weight.size(0)):
+        raise ValueError(f"embedding: padding_idx {padding_idx} outside "
+                         f"the {weight.size(0)} rows")
     y = F.embedding(ids, weight, padding_idx)
     return y if scale == 1.0 else y * scale
 
