@@ -74,60 +74,97 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
 // sorting them gives one order. Ids that take no part (padding, or outside
 // [0, V)) get the id V and end up behind all others.
 //
-// Tiles of kTile keys are sorted in LDS (bitonic); then runs are merged, up
-// to kMergeRuns at a time: a key's place in the merged run is its place in
-// its own run plus the number of smaller keys in each of the others, found by
-// bisection. That takes one launch for up to 32768 tokens, two up to 524288.
+// Within tiles of kTile keys a key's place is counted: the smaller ids in the
+// tile, and the equal ones before it. All pairs are compared, kTile for each
+// token, but over the whole chip and without a barrier in between: a bitonic
+// sort of a tile by one block took 15 us for any number of tokens, the count
+// takes 4. Then runs are merged, up to kMergeRuns at a time: a key's place in
+// the merged run is its place in its own run plus the number of smaller keys
+// in each of the others, one lane for each run and a bisection of dependent
+// loads once instead of 15 times. One merge does for up to 32768 tokens, two
+// for up to 524288.
 
 constexpr int kTile = 2048;
-constexpr int kSortThreads = 1024;
+constexpr int kRankThreads = 1024;
+constexpr int kRankKeys = 64;  // keys that a block places, one for each lane
 constexpr int kMergeRuns = 16;
 
-// The blocks behind the tiles' fill dW with zeros meanwhile: sorting is a
-// matter of latency on few CUs, filling one of bandwidth.
+// dW is filled with zeros by further blocks of the sorting launches, which
+// leave memory idle; each writes kFillUnits units of 16 bytes.
+constexpr int kFillUnits = 4096;
+
+struct Fill {
+  u32x4* at;
+  int64_t units;
+};
+
+template <int kBlock>
+__device__ __forceinline__ void fill(const Fill& f, int64_t block) {
+  const int64_t begin = block * kFillUnits + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kFillUnits / kBlock; ++k)
+    if (begin + k * kBlock < f.units)
+      f.at[begin + k * kBlock] = u32x4{0, 0, 0, 0};
+}
+
 template <typename I>
-__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
+__global__ __launch_bounds__(kRankThreads) void embed_rank_kernel(
     const I* __restrict__ ids, uint64_t* __restrict__ keys, int64_t n,
-    int64_t vocab, int64_t padding, int tiles, uint16_t* __restrict__ zeros,
-    int64_t nzeros) {
-  __shared__ uint64_t s[kTile];
-  if (static_cast<int>(blockIdx.x) >= tiles) {
-    const int64_t step =
-        static_cast<int64_t>(gridDim.x - tiles) * kSortThreads;
-    const int64_t at = static_cast<int64_t>(blockIdx.x - tiles) * kSortThreads +
-                       threadIdx.x;
-    u32x4* wide = reinterpret_cast<u32x4*>(zeros);
-    for (int64_t i = at; i < nzeros / 8; i += step) wide[i] = u32x4{0, 0, 0, 0};
-    if (at < nzeros % 8) zeros[nzeros / 8 * 8 + at] = 0;
+    int64_t vocab, int64_t padding, int blocks, Fill f) {
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    fill<kRankThreads>(f, blockIdx.x - blocks);
     return;
   }
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
-  for (int i = threadIdx.x; i < kTile; i += kSortThreads) {
-    uint64_t key = ~0ull;
-    if (base + i < n) {
+  constexpr int kWaves = kRankThreads / 64;
+  constexpr int kPart = kTile / kWaves;  // keys that a wave compares with
+  __shared__ alignas(16) uint32_t s[kTile];
+  __shared__ int counts[kWaves][kRankKeys];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRankKeys;
+  const int64_t base = first / kTile * kTile;
+  const int len = static_cast<int>(min<int64_t>(kTile, n - base));
+  for (int i = threadIdx.x; i < kTile; i += kRankThreads) {
+    uint32_t key = ~0u;  // never smaller than another
+    if (i < len) {
       const int64_t id = static_cast<int64_t>(ids[base + i]);
-      const bool part = id >= 0 && id < vocab && id != padding;
-      key = static_cast<uint64_t>(part ? id : vocab) << 32 |
-            static_cast<uint32_t>(base + i);
+      key = static_cast<uint32_t>(
+          id >= 0 && id < vocab && id != padding ? id : vocab);
     }
     s[i] = key;
   }
   __syncthreads();
-  for (int k = 2; k <= kTile; k <<= 1) {
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int t = threadIdx.x; t < kTile / 2; t += kSortThreads) {
-        const int a = 2 * t - (t & (j - 1)), b = a + j;
-        const uint64_t x = s[a], y = s[b];
-        if ((x > y) == ((a & k) == 0)) {
-          s[a] = y;
-          s[b] = x;
-        }
-      }
-      __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int mine = static_cast<int>(first - base) + lane;
+  const uint32_t key = s[mine];
+  int count = 0;
+  const int from = wave * kPart, to = min(from + kPart, len);
+  const int own = static_cast<int>(first - base);
+  if (from + kPart <= own) {  // all before the block's keys: equal ones count
+    for (int j = from; j < to; j += 4) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(&s[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) count += k[e] <= key;
+    }
+  } else if (from >= own + kRankKeys) {  // all behind them (or past the end)
+    for (int j = from; j < to; j += 4) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(&s[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) count += k[e] < key;
+    }
+  } else {
+    for (int j = from; j < to; ++j) {
+      const uint32_t k = s[j];
+      count += k < key || (k == key && j < mine);
     }
   }
-  for (int i = threadIdx.x; i < kTile; i += kSortThreads)
-    if (base + i < n) keys[base + i] = s[i];
+  counts[wave][lane] = count;
+  __syncthreads();
+  if (wave == 0 && mine < len) {
+    int place = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) place += counts[w][lane];
+    keys[base + place] = static_cast<uint64_t>(key) << 32 |
+                         static_cast<uint32_t>(base + mine);
+  }
 }
 
 // Keys below `key` in the sorted run p[0..n).
@@ -146,20 +183,28 @@ __device__ __forceinline__ int64_t count_below(const uint64_t* p, int64_t n,
 
 __global__ __launch_bounds__(kThreads) void embed_merge_kernel(
     const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int64_t n,
-    int64_t run) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= n) return;
-  const uint64_t key = in[i];
+    int64_t run, int64_t blocks, Fill f) {
+  if (static_cast<int64_t>(blockIdx.x) >= blocks) {
+    fill<kThreads>(f, blockIdx.x - blocks);
+    return;
+  }
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) /
+                    kMergeRuns;
+  const int r = threadIdx.x % kMergeRuns;
+  const bool on = i < n;
+  const uint64_t key = on ? in[i] : 0;
   const int64_t group = i / (run * kMergeRuns) * (run * kMergeRuns);
   const int64_t mine = i / run * run;
-  int64_t place = group + (i - mine);
-  for (int r = 0; r < kMergeRuns; ++r) {
-    const int64_t start = group + r * run;
-    if (start >= n) break;
-    if (start != mine)
-      place += count_below(in + start, min(run, n - start), key);
-  }
-  out[place] = key;
+  const int64_t start = group + r * run;
+  int64_t place = 0;
+  if (on && start == mine)
+    place = group + (i - mine);
+  else if (on && start < n)
+    place = count_below(in + start, min(run, n - start), key);
+#pragma unroll
+  for (int off = kMergeRuns / 2; off > 0; off >>= 1)
+    place += __shfl_xor(place, off, 64);
+  if (on && r == 0) out[place] = key;
 }
 
 // ------------------------------------------------------------ summing rows
@@ -170,10 +215,16 @@ __global__ __launch_bounds__(kThreads) void embed_merge_kernel(
 // chunk's border go to fp32 partial sums (slot 0: the id came from the chunk
 // before; slot 1: it starts here and goes on), which a second kernel joins
 // in order.
+//
+// A chunk has 64 tokens at most: each lane loads one key, and reading them
+// from the lanes makes ids and row addresses uniform, so that changes of the
+// id are scalar branches and kRowsAhead rows are in flight.
 
 constexpr int kRowsAhead = 8;
+constexpr int kMaxChunk = 64;
 
-template <typename T>
+// kTail: rows that are no whole number of 16-byte vectors.
+template <typename T, bool kTail>
 __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
     const uint64_t* __restrict__ keys, const T* __restrict__ dy,
     T* __restrict__ dw, float* __restrict__ part, int64_t n, int64_t vocab,
@@ -181,70 +232,84 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
   constexpr int V = kVec<T>;
   const int lane = threadIdx.x & 63;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) +
-                       (threadIdx.x >> 6);
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t ci = unit / slices;
   if (ci >= nchunks) return;
   const int64_t c0 = (unit % slices) * 64 * V + lane * V;
   const int64_t begin = ci * chunk;
-  const int64_t end = min(begin + chunk, n);
-  const int width = c0 >= dim ? 0 : static_cast<int>(min<int64_t>(V, dim - c0));
+  const int len = static_cast<int>(min<int64_t>(chunk, n - begin));
+  const int width =
+      c0 >= dim ? 0 : static_cast<int>(min<int64_t>(V, dim - c0));
+
+  const uint64_t mine = lane < len ? keys[begin + lane] : ~0ull;
+  const uint32_t none = static_cast<uint32_t>(vocab);
+  const uint32_t before =
+      begin > 0 ? static_cast<uint32_t>(keys[begin - 1] >> 32) : none;
+  const uint32_t after = begin + len < n
+                             ? static_cast<uint32_t>(keys[begin + len] >> 32)
+                             : none;
+  auto id_at = [&](int k) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(
+        static_cast<int>(mine >> 32), k));
+  };
+  auto row_at = [&](int k) {
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_readlane(static_cast<int>(mine), k));
+  };
 
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  int64_t cur = static_cast<int64_t>(keys[begin] >> 32);
-  bool first = begin > 0 &&
-               static_cast<int64_t>(keys[begin - 1] >> 32) == cur;
+  uint32_t cur = id_at(0);
+  bool first = before == cur;
 
   auto flush = [&](bool goes_on) {
-    if (cur >= vocab || width == 0) return;
+    if (cur == none) return;
     if (first || goes_on) {
       float* p = part + (ci * 2 + (first ? 0 : 1)) * dim + c0;
+#pragma unroll
       for (int i = 0; i < V; ++i)
         if (i < width) p[i] = acc[i];
     } else {
-      T* p = dw + cur * dim + c0;
+      T* p = dw + static_cast<int64_t>(cur) * dim + c0;
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] *= scale;
       if (width == V) {
         store16(p, pack<T>(acc));
-      } else {
+      } else if (kTail) {
+#pragma unroll
         for (int i = 0; i < V; ++i)
           if (i < width) p[i] = static_cast<T>(acc[i]);
       }
     }
   };
 
-  for (int64_t p0 = begin; p0 < end; p0 += kRowsAhead) {
+  for (int p0 = 0; p0 < len; p0 += kRowsAhead) {
     u32x4 r[kRowsAhead];
-    int64_t id[kRowsAhead];
 #pragma unroll
     for (int k = 0; k < kRowsAhead; ++k) {
-      id[k] = vocab;
       r[k] = u32x4{0, 0, 0, 0};
-      if (p0 + k < end) {
-        const uint64_t key = keys[p0 + k];
-        id[k] = static_cast<int64_t>(key >> 32);
-        const T* src = dy + static_cast<int64_t>(key & 0xffffffffu) * dim + c0;
-        if (id[k] < vocab) {
-          if (width == V) {
-            r[k] = load16(src);
-          } else if (width > 0) {
-            T t[V] = {};
-            for (int i = 0; i < V; ++i)
-              if (i < width) t[i] = src[i];
-            __builtin_memcpy(&r[k], t, 16);
-          }
+      if (p0 + k < len && id_at(p0 + k) != none) {
+        const T* src = dy + static_cast<int64_t>(row_at(p0 + k)) * dim + c0;
+        if (width == V) {
+          r[k] = load16(src);
+        } else if (kTail && width > 0) {
+          T t[V] = {};
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (i < width) t[i] = src[i];
+          __builtin_memcpy(&r[k], t, 16);
         }
       }
     }
 #pragma unroll
     for (int k = 0; k < kRowsAhead; ++k) {
-      if (p0 + k < end) {
-        if (id[k] != cur) {
+      if (p0 + k < len) {
+        const uint32_t id = id_at(p0 + k);
+        if (id != cur) {
           flush(false);
           first = false;
-          cur = id[k];
+          cur = id;
 #pragma unroll
           for (int i = 0; i < V; ++i) acc[i] = 0.f;
         }
@@ -255,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
       }
     }
   }
-  flush(end < n && static_cast<int64_t>(keys[end] >> 32) == cur);
+  flush(after == cur);
 }
 
 // One block joins one chunk's slot 1 with the slots 0 behind it, if an id
@@ -305,13 +370,13 @@ struct SumPlan {
 };
 
 // Chunks are as long as still leaves about 4096 waves (4 for each SIMD), and
-// 8 to 256 tokens: a short chunk keeps few loads in flight, a long one leaves
+// 8 to 64 tokens: a short chunk keeps few loads in flight, a long one leaves
 // CUs idle.
 SumPlan sum_plan(int64_t n, int64_t dim, int vec) {
   SumPlan p;
   p.slices = static_cast<int>((dim + 64 * vec - 1) / (64 * vec));
   p.chunk = 8;
-  while (p.chunk < 256 && n / p.chunk * p.slices > 4096) p.chunk *= 2;
+  while (p.chunk < kMaxChunk && n / p.chunk * p.slices > 4096) p.chunk *= 2;
   p.nchunks = (n + p.chunk - 1) / p.chunk;
   return p;
 }
@@ -320,25 +385,45 @@ template <typename T, typename I>
 void bwd(const I* ids, const T* dy, T* dw, uint64_t* keys, float* part,
          int64_t n, int64_t vocab, int64_t dim, int64_t padding, float scale,
          hipStream_t stream) {
-  const int tiles = static_cast<int>((n + kTile - 1) / kTile);
-  const int64_t nzeros = vocab * dim * static_cast<int64_t>(sizeof(T) / 2);
-  const int fill = static_cast<int>(std::min<int64_t>(
-      1024, (nzeros / 8 + kSortThreads) / kSortThreads));
-  hipLaunchKernelGGL(embed_sort_kernel<I>, dim3(tiles + fill),
-                     dim3(kSortThreads), 0, stream, ids, keys, n, vocab,
-                     padding, tiles, reinterpret_cast<uint16_t*>(dw), nzeros);
+  // The allocation of dw is rounded up to 16 bytes for the fill.
+  int64_t left = (vocab * dim * static_cast<int64_t>(sizeof(T)) + 15) / 16;
+  int passes = 1;
+  for (int64_t run = kTile; run < n; run *= kMergeRuns) ++passes;
+  u32x4* at = reinterpret_cast<u32x4*>(dw);
+  auto next_fill = [&] {  // an equal share for each launch that is left
+    const int64_t blocks =
+        (left + kFillUnits * passes - 1) / (kFillUnits * passes);
+    const Fill f = {at, std::min(left, blocks * kFillUnits)};
+    at += f.units;
+    left -= f.units;
+    --passes;
+    return f;
+  };
+  auto fill_blocks = [](const Fill& f) {
+    return (f.units + kFillUnits - 1) / kFillUnits;
+  };
+  const int64_t ranks = (n + kRankKeys - 1) / kRankKeys;
+  Fill f = next_fill();
+  hipLaunchKernelGGL(embed_rank_kernel<I>,
+                     dim3(static_cast<unsigned>(ranks + fill_blocks(f))),
+                     dim3(kRankThreads), 0, stream, ids, keys, n, vocab,
+                     padding, static_cast<int>(ranks), f);
   if (n == 0) return;
   uint64_t* other = keys + n;
   for (int64_t run = kTile; run < n; run *= kMergeRuns) {
+    f = next_fill();
+    const int64_t blocks = (n * kMergeRuns + kThreads - 1) / kThreads;
     hipLaunchKernelGGL(embed_merge_kernel,
-                       dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, stream, keys, other, n, run);
+                       dim3(static_cast<unsigned>(blocks + fill_blocks(f))),
+                       dim3(kThreads), 0, stream, keys, other, n, run, blocks,
+                       f);
     std::swap(keys, other);
   }
   const SumPlan p = sum_plan(n, dim, kVec<T>);
   const int64_t units = p.nchunks * p.slices;
-  hipLaunchKernelGGL(embed_sum_kernel<T>,
-                     dim3(static_cast<unsigned>((units + 3) / 4)),
+  auto* sum = dim % kVec<T> ? &embed_sum_kernel<T, true>
+                            : &embed_sum_kernel<T, false>;
+  hipLaunchKernelGGL(sum, dim3(static_cast<unsigned>((units + 3) / 4)),
                      dim3(kThreads), 0, stream, keys, dy, dw, part, n, vocab,
                      dim, p.chunk, p.nchunks, p.slices, scale);
   if (p.nchunks > 1)

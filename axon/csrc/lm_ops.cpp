@@ -69,8 +69,12 @@ at::Tensor embed_bwd(const at::Tensor& ids, const at::Tensor& dy_in,
   const Guard guard(dy_in.device());
   const at::Tensor dy = dy_in.contiguous();
   const int64_t n = ids.numel(), dim = dy.size(-1);
-  at::Tensor dw = at::empty({vocab, dim}, dy.options());
-  if (dw.numel() == 0) return dw;
+  // Whole units of 16 bytes, as the kernels fill it.
+  const int64_t unit = 16 / static_cast<int64_t>(dy.element_size());
+  at::Tensor dw =
+      at::empty({(vocab * dim + unit - 1) / unit * unit}, dy.options());
+  if (dw.numel() == 0) return dw.view({vocab, dim});
+  dw = dw.as_strided({vocab, dim}, {dim, 1});
   at::Tensor keys = at::empty({2 * n}, ids.options().dtype(at::kLong));
   at::Tensor part =
       at::empty({embed_part_floats(n, dim, static_cast<int>(dy.element_size()))},
