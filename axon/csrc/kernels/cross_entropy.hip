@@ -10,6 +10,7 @@
 // logits' size is kept between. Rows whose label is ignored are not read, and
 // their gradient is zeros.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 #include "lm_util.h"
@@ -51,6 +52,28 @@ __device__ __forceinline__ Stat join(Stat a, Stat b) {
   return {m, a.s * exp_of(a.m - m) + b.s * exp_of(b.m - m), a.x + b.x};
 }
 
+// Values before the next border of a 128-byte line, which a group handles one
+// by one, so that its vectors lie on such borders: rows of an odd length
+// start anywhere. (32768 rows of 30522 bf16, both passes past the caches: 1241
+// us with vectors from each row's start, 1021 with this.)
+template <typename T>
+__device__ __forceinline__ int head_of(const T* p, int len) {
+  const uintptr_t past = reinterpret_cast<uintptr_t>(p) & 127;
+  return min(len, static_cast<int>((128 - past & 127) / sizeof(T)));
+}
+
+template <bool kOnce, typename T>
+__device__ __forceinline__ u32x4 load(const T* p) {
+  return kOnce ? load16_once(p) : load16(p);
+}
+template <bool kOnce, typename T>
+__device__ __forceinline__ void store(T* p, u32x4 r) {
+  if (kOnce)
+    store16_once(p, r);
+  else
+    store16(p, r);
+}
+
 // Row r of logits [outer, inner, V] with strides; labels are dense.
 struct Rows {
   int64_t inner, stride_outer, stride_inner;
@@ -80,7 +103,8 @@ template <typename T, int G, bool kSmooth, bool kWhole>
 __global__ __launch_bounds__(kThreads) void ce_stat_kernel(
     const T* __restrict__ x, Rows rows, const int64_t* __restrict__ target,
     int64_t ignore, int64_t n, int64_t vocab, int64_t seg_len, int segs,
-    float small, float eps, Stat* __restrict__ stat, float2* __restrict__ kept,
+    int64_t once_rows, float small, float eps, float unlabelled,
+    Stat* __restrict__ stat, float2* __restrict__ kept,
     float* __restrict__ losses) {
   constexpr int V = kVec<T>;
   constexpr int kAhead = 4;
@@ -90,16 +114,23 @@ __global__ __launch_bounds__(kThreads) void ce_stat_kernel(
   const int64_t label = row < n ? target[row] : ignore;
   const bool reads = label != ignore;
   const int t = threadIdx.x % G;
-  if (kWhole && !reads && t == 0 && row < n) losses[row] = 0.f;
+  if (kWhole && !reads && t == 0 && row < n) losses[row] = unlabelled;
   if (G == kThreads && !reads) return;
   const bool known = label >= 0 && label < vocab;
   Stat st = {kLowest, 0.f, 0.f};
   float xt = 0.f;
   if (reads) {
     const int64_t begin = kWhole ? 0 : unit % segs * seg_len;
-    const int64_t len = kWhole ? vocab : min(seg_len, vocab - begin);
+    const int len = static_cast<int>(kWhole ? vocab
+                                            : min(seg_len, vocab - begin));
     const T* p = x + rows.at(row) + begin;
     if (kWhole && known) xt = static_cast<float>(p[label]);
+    auto take_one = [&](float f) {
+      const float m = fmaxf(st.m, f);
+      st.s = st.s * exp_of(st.m - m) + exp_of(f - m);
+      if (kSmooth) st.x = fmaf(f, small, st.x);
+      st.m = m;
+    };
     auto take = [&](u32x4 r) {
       float f[V];
       unpack<T>(r, f);
@@ -115,23 +146,29 @@ __global__ __launch_bounds__(kThreads) void ce_stat_kernel(
       st.m = m;
       st.s = s;
     };
-    const int64_t full = len / V;
-    int64_t i = t;
-    for (; i + (kAhead - 1) * G < full; i += kAhead * G) {
-      u32x4 r[kAhead];
+    const int head = head_of(p, len);
+    for (int j = t; j < head; j += G) take_one(static_cast<float>(p[j]));
+    const T* body = p + head;
+    const int full = (len - head) / V;
+    auto vectors = [&](auto once) {
+      constexpr bool kOnce = decltype(once)::value;
+      int i = t;
+      for (; i + (kAhead - 1) * G < full; i += kAhead * G) {
+        u32x4 r[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) r[k] = load16(p + (i + k * G) * V);
+        for (int k = 0; k < kAhead; ++k)
+          r[k] = load<kOnce>(body + (i + k * G) * V);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) take(r[k]);
-    }
-    for (; i < full; i += G) take(load16(p + i * V));
-    for (int64_t j = full * V + t; j < len; j += G) {
-      const float f = static_cast<float>(p[j]);
-      const float m = fmaxf(st.m, f);
-      st.s = st.s * exp_of(st.m - m) + exp_of(f - m);
-      if (kSmooth) st.x = fmaf(f, small, st.x);
-      st.m = m;
-    }
+        for (int k = 0; k < kAhead; ++k) take(r[k]);
+      }
+      for (; i < full; i += G) take(load<kOnce>(body + i * V));
+    };
+    if (row < once_rows)
+      vectors(std::true_type{});
+    else
+      vectors(std::false_type{});
+    for (int j = head + full * V + t; j < len; j += G)
+      take_one(static_cast<float>(p[j]));
   }
 #pragma unroll
   for (int off = (G < 64 ? G : 64) / 2; off > 0; off >>= 1) {
@@ -161,13 +198,14 @@ __global__ __launch_bounds__(kThreads) void ce_stat_kernel(
 __global__ __launch_bounds__(kThreads) void ce_join_kernel(
     const void* __restrict__ x, int dtype, Rows rows,
     const int64_t* __restrict__ target, int64_t ignore, int64_t n,
-    int64_t vocab, int segs, float eps, const Stat* __restrict__ stat,
-    float2* __restrict__ kept, float* __restrict__ losses) {
+    int64_t vocab, int segs, float eps, float unlabelled,
+    const Stat* __restrict__ stat, float2* __restrict__ kept,
+    float* __restrict__ losses) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (row >= n) return;
   const int64_t t = target[row];
   if (t == ignore) {
-    losses[row] = 0.f;
+    losses[row] = unlabelled;
     return;
   }
   const bool known = t >= 0 && t < vocab;
@@ -185,22 +223,31 @@ __global__ __launch_bounds__(kThreads) void ce_join_kernel(
 
 // Sums the rows' losses and counts the labels, in 64 bits: one block for up
 // to kSumRows rows, else partial sums of that many each and a second launch
-// over those (`sums` in, `losses` null).
+// over those (`in`). A row without a label holds kUnlabelled: no loss is
+// -inf, since S >= 1 and m >= x_t wherever the loss is a number.
 constexpr int kSumThreads = 1024;
 constexpr int64_t kSumRows = 16384;
+constexpr float kUnlabelled = -__builtin_inff();
 
 __global__ __launch_bounds__(kSumThreads) void ce_sum_kernel(
-    const float* __restrict__ losses, const int64_t* __restrict__ target,
-    int64_t ignore, int64_t n, const double* __restrict__ in,
+    const float* __restrict__ losses, int64_t n, const double* __restrict__ in,
     double* __restrict__ out, bool mean, float* __restrict__ loss,
     float* __restrict__ factor) {
   double sum = 0.0, count = 0.0;
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * kSumRows;
   const int64_t end = min(n, begin + kSumRows);
-#pragma unroll 4
-  for (int64_t i = begin + threadIdx.x; i < end; i += kSumThreads) {
-    sum += in ? in[2 * i] : static_cast<double>(losses[i]);
-    count += in ? in[2 * i + 1] : (target[i] != ignore ? 1.0 : 0.0);
+  if (in) {
+    for (int64_t i = begin + threadIdx.x; i < end; i += kSumThreads) {
+      sum += in[2 * i];
+      count += in[2 * i + 1];
+    }
+  } else {
+#pragma unroll 8
+    for (int64_t i = begin + threadIdx.x; i < end; i += kSumThreads) {
+      const float l = losses[i];
+      sum += l == kUnlabelled ? 0.0 : static_cast<double>(l);
+      count += l == kUnlabelled ? 0.0 : 1.0;
+    }
   }
   __shared__ double lds[2][kSumThreads / 64];
   sum = wave_sum(sum);
@@ -225,65 +272,85 @@ __global__ __launch_bounds__(kSumThreads) void ce_sum_kernel(
   }
 }
 
-template <typename T, int G>
+template <typename T, int G, bool kOnce>
 __global__ __launch_bounds__(kThreads) void ce_grad_kernel(
     const T* __restrict__ x, Rows rows, const int64_t* __restrict__ target,
     int64_t ignore, int64_t n, int64_t vocab, int64_t seg_len, int segs,
-    float eps, const float2* __restrict__ kept, const float* __restrict__ gout,
+    int64_t once_rows, float eps, const float2* __restrict__ kept, const float* __restrict__ gout,
     int gstride, const float* __restrict__ factor, T* __restrict__ dx) {
   constexpr int V = kVec<T>;
   constexpr int kAhead = 4;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / G) +
-                       threadIdx.x / G;
+  // Last rows first: they are in the cache.
+  const int64_t unit =
+      static_cast<int64_t>(gridDim.x - 1 - blockIdx.x) * (kThreads / G) +
+      threadIdx.x / G;
   const int64_t row = unit / segs;
   if (row >= n) return;
   const int t = threadIdx.x % G;
   const int64_t begin = unit % segs * seg_len;
-  const int64_t len = min(seg_len, vocab - begin);
-  const int64_t full = len / V;
+  const int len = static_cast<int>(min(seg_len, vocab - begin));
   T* q = dx + row * vocab + begin;
+  const int head = head_of(q, len);
+  const int full = (len - head) / V;
+  const int tail = head + full * V;
+  T* qbody = q + head;
   const int64_t label = target[row];
   if (label == ignore) {
-    for (int64_t i = t; i < full; i += G) store16(q + i * V, u32x4{0, 0, 0, 0});
-    for (int64_t j = full * V + t; j < len; j += G) q[j] = static_cast<T>(0.f);
+    const u32x4 zero = {0, 0, 0, 0};
+    for (int j = t; j < head; j += G) q[j] = static_cast<T>(0.f);
+    for (int i = t; i < full; i += G) store<kOnce>(qbody + i * V, zero);
+    for (int j = tail + t; j < len; j += G) q[j] = static_cast<T>(0.f);
     return;
   }
   const T* p = x + rows.at(row) + begin;
+  const T* body = p + head;
   float g = gout[row * gstride];
   if (factor) g *= *factor;
-  if (label < 0 || label >= vocab) g = __builtin_nanf("");
+  const bool known = label >= 0 && label < vocab;
+  if (!known) g = __builtin_nanf("");
   const float2 st = kept[row];
   const float scale = st.y * g;
   const float off = eps > 0.f ? g * eps / static_cast<float>(vocab) : 0.f;
   const float hit = g * (1.f - eps);
-  const int64_t at = label - begin;  // the label's place in this segment
-  auto value = [&](float f, int64_t j) {
-    float v = exp_of(f - st.x) * scale - off;
-    return j == at ? v - hit : v;
+  // The label's place in this segment, if it is here.
+  const int at = known && label >= begin && label - begin < len
+                     ? static_cast<int>(label - begin)
+                     : -1;
+  auto one = [&](int j) {
+    const float v = exp_of(static_cast<float>(p[j]) - st.x) * scale - off;
+    q[j] = static_cast<T>(j == at ? v - hit : v);
   };
-  int64_t i = t;
-  for (; i + (kAhead - 1) * G < full; i += kAhead * G) {
-    u32x4 r[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) r[k] = load16(p + (i + k * G) * V);
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      float f[V];
-      unpack<T>(r[k], f);
-#pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = value(f[e], (i + k * G) * V + e);
-      store16(q + (i + k * G) * V, pack<T>(f));
-    }
-  }
-  for (; i < full; i += G) {
+  auto put = [&](u32x4 r, int i) {
     float f[V];
-    unpack<T>(load16(p + i * V), f);
+    unpack<T>(r, f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = value(f[e], i * V + e);
-    store16(q + i * V, pack<T>(f));
-  }
-  for (int64_t j = full * V + t; j < len; j += G)
-    q[j] = static_cast<T>(value(static_cast<float>(p[j]), j));
+    for (int e = 0; e < V; ++e) f[e] = exp_of(f[e] - st.x) * scale - off;
+    const int in = at - head - i * V;
+    if (in >= 0 && in < V) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = e == in ? f[e] - hit : f[e];
+    }
+    store<kOnce>(qbody + i * V, pack<T>(f));
+  };
+  auto vectors = [&](auto once) {
+    constexpr bool kReadOnce = decltype(once)::value;
+    int i = t;
+    for (; i + (kAhead - 1) * G < full; i += kAhead * G) {
+      u32x4 r[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        r[k] = load<kReadOnce>(body + (i + k * G) * V);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) put(r[k], i + k * G);
+    }
+    for (; i < full; i += G) put(load<kReadOnce>(body + i * V), i);
+  };
+  for (int j = t; j < head; j += G) one(j);
+  if (kOnce && row < once_rows)
+    vectors(std::true_type{});
+  else
+    vectors(std::false_type{});
+  for (int j = tail + t; j < len; j += G) one(j);
 }
 
 // 16 lanes for a row of up to 128 logits, a wave for one of up to 1024, a
@@ -310,6 +377,21 @@ unsigned blocks_of(const Plan& p, int64_t n) {
   return static_cast<unsigned>((n * p.segs + per - 1) / per);
 }
 
+// Rows that go past the caches, in both passes, as all of the gradient does
+// then: the chip's last cache (256 MB) keeps the last kKeep bytes of the
+// logits from the forward to the backward pass, which takes the rows from the
+// last to the first; streaming the others through it would displace them.
+// Forward and backward of 4096 x 30528 bf16 (250 MB): all through the caches
+// 154 us, all past them 136, kKeep of 64, 128, 192 MB 135, 128, 122; of
+// 8192 x 128256 (2.1 GB): 1207, 1140, and 1131, 1125, 1116, 1096 in that order
+// of rows. Smaller logits are cached whole.
+constexpr int64_t kKeep = int64_t{192} << 20;
+
+int64_t once_rows_of(int64_t n, int64_t vocab, size_t size) {
+  return std::max<int64_t>(
+      0, n - kKeep / (vocab * static_cast<int64_t>(size)));
+}
+
 template <typename T, bool kSmooth>
 auto* stat_kernel(const Plan& p) {
   if (p.segs > 1) return &ce_stat_kernel<T, kThreads, kSmooth, false>;
@@ -320,12 +402,21 @@ auto* stat_kernel(const Plan& p) {
 
 template <typename T>
 void stat_pass(const Plan& p, const void* x, Rows rows, const int64_t* target,
-               int64_t ignore, int64_t n, int64_t vocab, float eps, Stat* stat,
-               float2* kept, float* losses, hipStream_t stream) {
+               int64_t ignore, int64_t n, int64_t vocab, float eps,
+               float unlabelled, Stat* stat, float2* kept, float* losses,
+               hipStream_t stream) {
   auto* k = eps > 0.f ? stat_kernel<T, true>(p) : stat_kernel<T, false>(p);
   hipLaunchKernelGGL(k, dim3(blocks_of(p, n)), dim3(kThreads), 0, stream,
                      static_cast<const T*>(x), rows, target, ignore, n, vocab,
-                     p.seg_len, p.segs, down(vocab), eps, stat, kept, losses);
+                     p.seg_len, p.segs, once_rows_of(n, vocab, sizeof(T)),
+                     down(vocab), eps, unlabelled, stat, kept, losses);
+}
+
+template <typename T, bool kOnce>
+auto* grad_kernel(const Plan& p) {
+  return p.group == 16   ? &ce_grad_kernel<T, 16, kOnce>
+         : p.group == 64 ? &ce_grad_kernel<T, 64, kOnce>
+                         : &ce_grad_kernel<T, kThreads, kOnce>;
 }
 
 template <typename T>
@@ -333,12 +424,11 @@ void grad_pass(const Plan& p, const void* x, Rows rows, const int64_t* target,
                int64_t ignore, int64_t n, int64_t vocab, float eps,
                const float2* kept, const float* gout, int gstride,
                const float* factor, void* dx, hipStream_t stream) {
-  auto* k = p.group == 16   ? &ce_grad_kernel<T, 16>
-            : p.group == 64 ? &ce_grad_kernel<T, 64>
-                            : &ce_grad_kernel<T, kThreads>;
+  const int64_t once = once_rows_of(n, vocab, sizeof(T));
+  auto* k = once ? grad_kernel<T, true>(p) : grad_kernel<T, false>(p);
   hipLaunchKernelGGL(k, dim3(blocks_of(p, n)), dim3(kThreads), 0, stream,
                      static_cast<const T*>(x), rows, target, ignore, n, vocab,
-                     p.seg_len, p.segs, eps, kept, gout, gstride, factor,
+                     p.seg_len, p.segs, once, eps, kept, gout, gstride, factor,
                      static_cast<T*>(dx));
 }
 
@@ -368,28 +458,29 @@ void launch_ce_fwd(int dtype, const void* x, int64_t inner,
   float* losses = reduction ? own : loss;
   Stat* stat = reinterpret_cast<Stat*>(own + n);
   float2* kept = reinterpret_cast<float2*>(kept_);
+  const float unlabelled = reduction ? kUnlabelled : 0.f;
   if (n > 0) {
     auto* pass = dtype == kFloat  ? stat_pass<float>
                  : dtype == kHalf ? stat_pass<_Float16>
                                   : stat_pass<__bf16>;
-    pass(p, x, rows, target, ignore, n, vocab, eps, stat, kept, losses,
-         stream);
+    pass(p, x, rows, target, ignore, n, vocab, eps, unlabelled, stat, kept,
+         losses, stream);
     if (p.segs > 1)
       hipLaunchKernelGGL(ce_join_kernel,
                          dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)),
                          dim3(kThreads), 0, stream, x, dtype, rows, target,
-                         ignore, n, vocab, p.segs, eps, stat, kept, losses);
+                         ignore, n, vocab, p.segs, eps, unlabelled, stat, kept,
+                         losses);
   }
   if (!reduction) return;
   const bool mean = reduction == 1;
   hipLaunchKernelGGL(ce_sum_kernel, dim3(static_cast<unsigned>(
                          std::max<int64_t>(1, blocks))),
-                     dim3(kSumThreads), 0, stream, losses, target, ignore, n,
-                     nullptr, blocks > 1 ? sums : nullptr, mean, loss, factor);
+                     dim3(kSumThreads), 0, stream, losses, n, nullptr,
+                     blocks > 1 ? sums : nullptr, mean, loss, factor);
   if (blocks > 1)
     hipLaunchKernelGGL(ce_sum_kernel, dim3(1), dim3(kSumThreads), 0, stream,
-                       nullptr, nullptr, ignore, blocks, sums, nullptr, mean,
-                       loss, factor);
+                       nullptr, blocks, sums, nullptr, mean, loss, factor);
 }
 
 void launch_ce_bwd(int dtype, const void* x, int64_t inner,

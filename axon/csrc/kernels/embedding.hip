@@ -74,11 +74,12 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
 // sorting them gives one order. Ids that take no part (padding, or outside
 // [0, V)) get the id V and end up behind all others.
 //
-// Within tiles of kTile keys a key's place is counted: the smaller ids in the
-// tile, and the equal ones before it. All pairs are compared, kTile for each
+// Within tiles a key's place is counted: the smaller ids in the tile, and the
+// equal ones before it. All pairs are compared, a tile's length for each
 // token, but over the whole chip and without a barrier in between: a bitonic
-// sort of a tile by one block took 15 us for any number of tokens, the count
-// takes 4. Then runs are merged, up to kMergeRuns at a time: a key's place in
+// sort of 2048 keys by one block took 15 us, the count takes 5. (A tile of
+// 8192 would save their merge, but took 22 us instead of 9 and 10.) Then runs
+// are merged, up to kMergeRuns at a time: a key's place in
 // the merged run is its place in its own run plus the number of smaller keys
 // in each of the others, one lane for each run and a bisection of dependent
 // loads once instead of 15 times. One merge does for up to 32768 tokens, two
@@ -96,7 +97,25 @@ constexpr int kFillUnits = 4096;
 struct Fill {
   u32x4* at;
   int64_t units;
+  __host__ __device__ int64_t blocks() const {
+    return (units + kFillUnits - 1) / kFillUnits;
+  }
 };
+
+// Of the launch's blocks, every second one fills until the others (or the
+// fill) run out: blocks start in order, and either kind alone would take all
+// CUs first. Returns this block's number among its kind; *fills says which.
+__device__ __forceinline__ int64_t kind_of(int64_t block, int64_t others,
+                                           int64_t fills_in_all,
+                                           bool* fills) {
+  const int64_t pairs = min(others, fills_in_all);
+  if (block < 2 * pairs) {
+    *fills = block & 1;
+    return block >> 1;
+  }
+  *fills = fills_in_all > others;
+  return block - pairs;
+}
 
 template <int kBlock>
 __device__ __forceinline__ void fill(const Fill& f, int64_t block) {
@@ -110,16 +129,18 @@ __device__ __forceinline__ void fill(const Fill& f, int64_t block) {
 template <typename I>
 __global__ __launch_bounds__(kRankThreads) void embed_rank_kernel(
     const I* __restrict__ ids, uint64_t* __restrict__ keys, int64_t n,
-    int64_t vocab, int64_t padding, int blocks, Fill f) {
-  if (static_cast<int>(blockIdx.x) >= blocks) {
-    fill<kRankThreads>(f, blockIdx.x - blocks);
+    int64_t vocab, int64_t padding, int64_t blocks, Fill f) {
+  bool fills;
+  const int64_t block = kind_of(blockIdx.x, blocks, f.blocks(), &fills);
+  if (fills) {
+    fill<kRankThreads>(f, block);
     return;
   }
   constexpr int kWaves = kRankThreads / 64;
   constexpr int kPart = kTile / kWaves;  // keys that a wave compares with
   __shared__ alignas(16) uint32_t s[kTile];
   __shared__ int counts[kWaves][kRankKeys];
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRankKeys;
+  const int64_t first = block * kRankKeys;
   const int64_t base = first / kTile * kTile;
   const int len = static_cast<int>(min<int64_t>(kTile, n - base));
   for (int i = threadIdx.x; i < kTile; i += kRankThreads) {
@@ -138,22 +159,24 @@ __global__ __launch_bounds__(kRankThreads) void embed_rank_kernel(
   int count = 0;
   const int from = wave * kPart, to = min(from + kPart, len);
   const int own = static_cast<int>(first - base);
-  if (from + kPart <= own) {  // all before the block's keys: equal ones count
+  // An equal id counts if it stands before: k <= key is k < key + 1. Waves
+  // whose keys all stand on one side of the block's own need no comparison
+  // of positions.
+  const bool mixed = from < own + kRankKeys && from + kPart > own;
+  const uint32_t bound = key + (from < own ? 1 : 0);
+  if (!mixed) {
+#pragma unroll 4
     for (int j = from; j < to; j += 4) {
       const u32x4 k = *reinterpret_cast<const u32x4*>(&s[j]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) count += k[e] <= key;
-    }
-  } else if (from >= own + kRankKeys) {  // all behind them (or past the end)
-    for (int j = from; j < to; j += 4) {
-      const u32x4 k = *reinterpret_cast<const u32x4*>(&s[j]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) count += k[e] < key;
+      for (int e = 0; e < 4; ++e) count += k[e] < bound;
     }
   } else {
-    for (int j = from; j < to; ++j) {
-      const uint32_t k = s[j];
-      count += k < key || (k == key && j < mine);
+#pragma unroll 4
+    for (int j = from; j < to; j += 4) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(&s[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) count += k[e] < key + (j + e < mine ? 1 : 0);
     }
   }
   counts[wave][lane] = count;
@@ -184,12 +207,13 @@ __device__ __forceinline__ int64_t count_below(const uint64_t* p, int64_t n,
 __global__ __launch_bounds__(kThreads) void embed_merge_kernel(
     const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int64_t n,
     int64_t run, int64_t blocks, Fill f) {
-  if (static_cast<int64_t>(blockIdx.x) >= blocks) {
-    fill<kThreads>(f, blockIdx.x - blocks);
+  bool fills;
+  const int64_t block = kind_of(blockIdx.x, blocks, f.blocks(), &fills);
+  if (fills) {
+    fill<kThreads>(f, block);
     return;
   }
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) /
-                    kMergeRuns;
+  const int64_t i = (block * kThreads + threadIdx.x) / kMergeRuns;
   const int r = threadIdx.x % kMergeRuns;
   const bool on = i < n;
   const uint64_t key = on ? in[i] : 0;
@@ -267,9 +291,14 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
     if (cur == none) return;
     if (first || goes_on) {
       float* p = part + (ci * 2 + (first ? 0 : 1)) * dim + c0;
+      if (width == V) {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < width) p[i] = acc[i];
+        for (int i = 0; i < V; i += 4) store16(p + i, pack<float>(acc + i));
+      } else if (kTail) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i < width) p[i] = acc[i];
+      }
     } else {
       T* p = dw + static_cast<int64_t>(cur) * dim + c0;
 #pragma unroll
@@ -292,7 +321,7 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
       if (p0 + k < len && id_at(p0 + k) != none) {
         const T* src = dy + static_cast<int64_t>(row_at(p0 + k)) * dim + c0;
         if (width == V) {
-          r[k] = load16(src);
+          r[k] = load16_once(src);
         } else if (kTail && width > 0) {
           T t[V] = {};
 #pragma unroll
@@ -325,43 +354,59 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
 
 // One block joins one chunk's slot 1 with the slots 0 behind it, if an id
 // starts in that chunk and goes on: its four waves take every fourth chunk
-// and are summed in order.
+// and are summed in order. Where the id ends is seen from the first keys of
+// the next 64 chunks, one for each lane, and found by bisection only behind
+// those.
+constexpr int kJoinCols = 4;  // columns of a lane
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void embed_join_kernel(
     const uint64_t* __restrict__ keys, const float* __restrict__ part,
     T* __restrict__ dw, int64_t n, int64_t vocab, int64_t dim, int chunk,
     float scale) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t ci = blockIdx.x;
   const int64_t begin = ci * chunk, end = begin + chunk;
   if (end >= n) return;
-  const int64_t id = static_cast<int64_t>(keys[end] >> 32);
-  if (id >= vocab || static_cast<int64_t>(keys[end - 1] >> 32) != id) return;
-  // Starts it here? Else an earlier chunk joins it.
-  if (begin > 0 && static_cast<int64_t>(keys[begin] >> 32) == id &&
-      static_cast<int64_t>(keys[begin - 1] >> 32) == id)
-    return;
-  const uint64_t after = static_cast<uint64_t>(id + 1) << 32;
-  const int64_t last =
-      (end + count_below(keys + end, n - end, after) - 1) / chunk;
-  __shared__ float s[kThreads / 64][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t c = static_cast<int64_t>(blockIdx.y) * 64 + lane;
-  float acc = 0.f;
-  if (c < dim) {
-    if (wave == 0) acc = part[(ci * 2 + 1) * dim + c];
-#pragma unroll 4
-    for (int64_t k = ci + 1 + wave; k <= last; k += kThreads / 64)
-      acc += part[k * 2 * dim + c];
+  const int64_t at = min(end + static_cast<int64_t>(lane) * chunk, n - 1);
+  const uint32_t next = static_cast<uint32_t>(keys[at] >> 32);
+  const uint32_t id = __builtin_amdgcn_readfirstlane(next);
+  const uint32_t before = static_cast<uint32_t>(keys[end - 1] >> 32);
+  const uint32_t earlier =
+      static_cast<uint32_t>(keys[begin > 0 ? begin - 1 : 0] >> 32);
+  // Does it start here? Else an earlier chunk joins it.
+  if (id >= vocab || before != id || (begin > 0 && earlier == id)) return;
+  // Chunk ci + l is reached if its first key has the id.
+  const uint64_t on =
+      __ballot(next == id && end + static_cast<int64_t>(lane) * chunk < n);
+  int64_t last = ci + __builtin_ctzll(~on | (1ull << 63));
+  if (on == ~0ull) {
+    const uint64_t after = static_cast<uint64_t>(id) + 1 << 32;
+    last = (end + count_below(keys + end, n - end, after) - 1) / chunk;
   }
-  s[wave][lane] = acc;
+  __shared__ float s[kThreads / 64][kJoinCols][64];
+  const int64_t c0 = static_cast<int64_t>(blockIdx.y) * 64 * kJoinCols + lane;
+  float acc[kJoinCols] = {};
+#pragma unroll 4
+  for (int64_t k = ci + wave; k <= last; k += kThreads / 64) {
+    const float* p = part + (k * 2 + (k == ci ? 1 : 0)) * dim;
+#pragma unroll
+    for (int i = 0; i < kJoinCols; ++i)
+      if (c0 + i * 64 < dim) acc[i] += p[c0 + i * 64];
+  }
+#pragma unroll
+  for (int i = 0; i < kJoinCols; ++i) s[wave][i][lane] = acc[i];
   __syncthreads();
-  if (wave == 0 && c < dim) {
+  // Wave w finishes column w of each lane.
+  const int64_t c = c0 + wave * 64;
+  if (c < dim) {
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) sum += s[w][lane];
+    for (int w = 0; w < kThreads / 64; ++w) sum += s[w][wave][lane];
     dw[id * dim + c] = static_cast<T>(sum * scale);
   }
 }
+static_assert(kJoinCols == kThreads / 64, "a wave for each column");
 
 struct SumPlan {
   int chunk;
@@ -369,14 +414,15 @@ struct SumPlan {
   int slices;
 };
 
-// Chunks are as long as still leaves about 4096 waves (4 for each SIMD), and
-// 8 to 64 tokens: a short chunk keeps few loads in flight, a long one leaves
-// CUs idle.
+// Chunks are as long as still leaves about 1024 waves (one for each SIMD), and
+// 8 to 64 tokens. Shorter ones leave the sums' time as it is and make more
+// rows to join: for 8192 tokens of 1024 bf16 values, chunks of 8, 16 and 32
+// took 7.6 + 14.3, 8.4 + 8.1 and 11.8 + 5.7 us (sums + join).
 SumPlan sum_plan(int64_t n, int64_t dim, int vec) {
   SumPlan p;
   p.slices = static_cast<int>((dim + 64 * vec - 1) / (64 * vec));
   p.chunk = 8;
-  while (p.chunk < kMaxChunk && n / p.chunk * p.slices > 4096) p.chunk *= 2;
+  while (p.chunk < kMaxChunk && n / p.chunk * p.slices > 1024) p.chunk *= 2;
   p.nchunks = (n + p.chunk - 1) / p.chunk;
   return p;
 }
@@ -399,22 +445,19 @@ void bwd(const I* ids, const T* dy, T* dw, uint64_t* keys, float* part,
     --passes;
     return f;
   };
-  auto fill_blocks = [](const Fill& f) {
-    return (f.units + kFillUnits - 1) / kFillUnits;
-  };
   const int64_t ranks = (n + kRankKeys - 1) / kRankKeys;
   Fill f = next_fill();
   hipLaunchKernelGGL(embed_rank_kernel<I>,
-                     dim3(static_cast<unsigned>(ranks + fill_blocks(f))),
+                     dim3(static_cast<unsigned>(ranks + f.blocks())),
                      dim3(kRankThreads), 0, stream, ids, keys, n, vocab,
-                     padding, static_cast<int>(ranks), f);
+                     padding, ranks, f);
   if (n == 0) return;
   uint64_t* other = keys + n;
   for (int64_t run = kTile; run < n; run *= kMergeRuns) {
     f = next_fill();
     const int64_t blocks = (n * kMergeRuns + kThreads - 1) / kThreads;
     hipLaunchKernelGGL(embed_merge_kernel,
-                       dim3(static_cast<unsigned>(blocks + fill_blocks(f))),
+                       dim3(static_cast<unsigned>(blocks + f.blocks())),
                        dim3(kThreads), 0, stream, keys, other, n, run, blocks,
                        f);
     std::swap(keys, other);
@@ -429,7 +472,8 @@ void bwd(const I* ids, const T* dy, T* dw, uint64_t* keys, float* part,
   if (p.nchunks > 1)
     hipLaunchKernelGGL(embed_join_kernel<T>,
                        dim3(static_cast<unsigned>(p.nchunks - 1),
-                            static_cast<unsigned>((dim + 63) / 64)),
+                            static_cast<unsigned>((dim + 64 * kJoinCols - 1) /
+                                                 (64 * kJoinCols))),
                        dim3(kThreads), 0, stream, keys, part, dw, n, vocab,
                        dim, p.chunk, scale);
 }

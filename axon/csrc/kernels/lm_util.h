@@ -37,6 +37,19 @@ __device__ __forceinline__ void store16(T* p, u32x4 r) {
   __builtin_memcpy(p, &r, 16);
 }
 
+// The same for data that is read or written once: it goes past the caches
+// without displacing what is in them.
+template <typename T>
+__device__ __forceinline__ u32x4 load16_once(const T* p) {
+  using Any = u32x4 __attribute__((aligned(sizeof(T))));
+  return __builtin_nontemporal_load(reinterpret_cast<const Any*>(p));
+}
+template <typename T>
+__device__ __forceinline__ void store16_once(T* p, u32x4 r) {
+  using Any = u32x4 __attribute__((aligned(sizeof(T))));
+  __builtin_nontemporal_store(r, reinterpret_cast<Any*>(p));
+}
+
 template <typename T>
 __device__ __forceinline__ void unpack(u32x4 r, float* f);
 template <>

@@ -259,9 +259,11 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
                     ", logits on ", logits.device());
   TORCH_CHECK_TYPE(float_type(logits),
                    "cross_entropy: logits must be float, half or bfloat16");
-  // The partial sums of more rows would take a third launch.
-  TORCH_CHECK_VALUE(target.numel() < (int64_t{1} << 28),
-                    "cross_entropy: too many rows");
+  // The partial sums of more rows would take a third launch; places within a
+  // row are counted in 32 bits.
+  TORCH_CHECK_VALUE(target.numel() < (int64_t{1} << 28) &&
+                        logits.size(-1) < (int64_t{1} << 30),
+                    "cross_entropy: fewer than 2^28 rows and 2^30 classes");
   check_no_tangent(logits, "cross_entropy");
   const Guard guard(logits.device());
   // With the caller's autograd: the gradient goes back through these.
