@@ -12,11 +12,11 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
 #include <mutex>
-#include <unordered_map>
 
 #include "kernels/grad_norm.h"
 #include "kernels/kernels.h"
@@ -326,45 +326,51 @@ struct Grads {
 Grads collect(const std::vector<at::Tensor>& ts, bool written) {
   Grads g;
   TORCH_CHECK_VALUE(!ts.empty(), "grad norm: no tensors");
-  struct Span {
-    const char *begin, *end;
-  };
-  std::vector<Span> spans;  // of the dense tensors
-  std::unordered_multimap<const void*, size_t> seen;
-  for (size_t i = 0; i < ts.size(); ++i) {
-    const at::Tensor& t = ts[i];
+  for (const at::Tensor& t : ts)
     TORCH_CHECK_VALUE(t.is_cuda() && t.layout() == at::kStrided &&
                           float_type(t) && t.device() == ts[0].device(),
                       "grad norm: tensors must be dense float/half/bfloat16 "
                       "on one GPU");
-    if (t.numel() == 0) continue;
-    const auto alike = seen.equal_range(t.data_ptr());
-    if (std::any_of(alike.first, alike.second, [&](const auto& e) {
-          const at::Tensor& o = ts[e.second];
-          return o.sizes() == t.sizes() && o.strides() == t.strides() &&
-                 o.scalar_type() == t.scalar_type();
-        }))
+  // By address: equal tensors are neighbours then (of those that start at one
+  // place, few as they are, each is compared with each).
+  std::vector<std::pair<const char*, size_t>> order;
+  order.reserve(ts.size());
+  for (size_t i = 0; i < ts.size(); ++i)
+    if (ts[i].numel())
+      order.emplace_back(static_cast<const char*>(ts[i].data_ptr()), i);
+  std::sort(order.begin(), order.end());
+  std::vector<char> skip(ts.size(), 0);
+  const char* dense_end = nullptr;
+  for (size_t k = 0, same = 0; k < order.size(); ++k) {
+    const at::Tensor& t = ts[order[k].second];
+    if (order[k].first != order[same].first) same = k;
+    for (size_t j = same; j < k && !skip[order[k].second]; ++j) {
+      const at::Tensor& o = ts[order[j].second];
+      skip[order[k].second] = o.sizes() == t.sizes() &&
+                              o.strides() == t.strides() &&
+                              o.scalar_type() == t.scalar_type();
+    }
+    if (skip[order[k].second] || !written) continue;
+    if (!t.is_non_overlapping_and_dense()) {
+      at::assert_no_internal_overlap(t);
       continue;
-    seen.emplace(t.data_ptr(), i);
+    }
+    // Two blocks would scale the same value. (A strided tensor's copy holds
+    // the values from before; writing it back gives the same ones.)
+    TORCH_CHECK_VALUE(order[k].first >= dense_end,
+                      "grad norm: gradients share memory in part");
+    dense_end = order[k].first + t.nbytes();
+  }
+  g.dense.reserve(ts.size());
+  for (size_t i = 0; i < ts.size(); ++i) {
+    const at::Tensor& t = ts[i];
+    if (!t.numel() || skip[i]) continue;
     if (t.is_non_overlapping_and_dense()) {
-      const char* p = static_cast<const char*>(t.data_ptr());
-      spans.push_back({p, p + t.nbytes()});
       g.dense.push_back(t);
     } else {
-      if (written) at::assert_no_internal_overlap(t);
       g.strided.emplace_back(t, g.dense.size());
       g.dense.push_back(t.contiguous());
     }
-  }
-  if (written) {
-    // Two blocks would scale the same value. (A strided tensor's copy holds
-    // the values from before; writing it back gives the same ones.)
-    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) {
-      return a.begin < b.begin;
-    });
-    for (size_t i = 1; i < spans.size(); ++i)
-      TORCH_CHECK_VALUE(spans[i].begin >= spans[i - 1].end,
-                        "grad norm: gradients share memory in part");
   }
   return g;
 }
@@ -448,6 +454,38 @@ at::Tensor grad_clip_(const std::vector<at::Tensor>& ts, int64_t type,
   return out;
 }
 
+// The gradients of lists of parameters, read here rather than in Python:
+// that takes longer than the kernels where there are hundreds of small ones.
+// False where one is not a float/half/bfloat16 tensor on the first one's GPU.
+bool param_grads(const pybind11::list& lists, std::vector<at::Tensor>& grads) {
+  for (const auto& list : lists) {
+    if (!PyList_Check(list.ptr())) return false;
+    const Py_ssize_t n = PyList_GET_SIZE(list.ptr());
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* o = PyList_GET_ITEM(list.ptr(), i);
+      if (!THPVariable_Check(o)) return false;
+      const at::Tensor& g = THPVariable_Unpack(o).grad();
+      if (!g.defined()) continue;
+      if (!g.is_cuda() || g.layout() != at::kStrided || !float_type(g) ||
+          (!grads.empty() && g.device() != grads[0].device()))
+        return false;
+      grads.push_back(g);
+    }
+  }
+  return true;
+}
+
+// For lists of parameters: (norm, factor) as fp32[2], None where none has a
+// gradient, False where the general path has to take them.
+pybind11::object param_grad_norm(const pybind11::list& lists, int64_t type,
+                                 double max_norm, bool clip) {
+  std::vector<at::Tensor> grads;
+  if (!param_grads(lists, grads)) return pybind11::bool_(false);
+  if (grads.empty()) return pybind11::none();
+  return pybind11::cast(clip ? grad_clip_(grads, type, max_norm)
+                             : grad_norm(grads, type, max_norm));
+}
+
 void grad_scale_(const std::vector<at::Tensor>& ts, const at::Tensor& factor) {
   const Grads g = collect(ts, true);
   TORCH_CHECK(factor.device() == ts[0].device() && factor.numel() == 1 &&
@@ -467,9 +505,9 @@ void register_lm(pybind11::module_& m) {
         py::arg("reduction"));
   m.def("grad_norm", &grad_norm, py::arg("tensors"), py::arg("type"),
         py::arg("max_norm"));
+  m.def("param_grad_norm", &param_grad_norm, py::arg("lists"),
+        py::arg("type"), py::arg("max_norm"), py::arg("clip"));
   m.def("grad_scale_", &grad_scale_, py::arg("tensors"), py::arg("factor"));
-  m.def("grad_clip_", &grad_clip_, py::arg("tensors"), py::arg("type"),
-        py::arg("max_norm"));
 }
 
 }  // namespace axon

@@ -4,7 +4,12 @@
 #include <torch/extension.h>
 
 #include <ATen/hip/HIPContext.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
 
 #include "kernels/optimizers.h"
 
@@ -34,6 +39,7 @@ ChunkPlan build_chunks(const std::vector<at::Tensor>& ps,
   for (auto& p : ps) total += p.numel();
   int64_t ce = pick_chunk_elems(total);
   std::vector<OptChunk> chunks;
+  chunks.reserve(ps.size() + total / ce);
   int64_t uoff = 0;
   for (size_t t = 0; t < ps.size(); ++t) {
     auto& p = ps[t];
@@ -165,9 +171,112 @@ void fused_lamb(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                            static_cast<const float*>(norms.data_ptr()), stream);
 }
 
+// ---------------------------------------------------------------- one group
+//
+// The work of a whole parameter group in one call: with hundreds of small
+// parameters the step is a matter of the time that the host takes for each.
+
+struct AdamLists {
+  std::vector<at::Tensor> ps, gs, ms, vs, steps;
+};
+
+// Reads the group's tensors into `l`; false where the general path has to
+// look at them first: state that is missing or of another layout or type, a
+// step count that is not one float on the CPU, anything not on one GPU.
+bool read_adam_group(PyObject* params, PyObject* state, AdamLists& l) {
+  static PyObject* const k_step = PyUnicode_InternFromString("step");
+  static PyObject* const k_m = PyUnicode_InternFromString("exp_avg");
+  static PyObject* const k_v = PyUnicode_InternFromString("exp_avg_sq");
+  if (!PyList_Check(params) || !PyDict_Check(state)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(params);
+  for (auto* v : {&l.ps, &l.gs, &l.ms, &l.vs, &l.steps}) v->reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(params, i);
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor& p = THPVariable_Unpack(o);
+    const at::Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    PyObject* st = PyDict_GetItemWithError(state, o);
+    if (!st && PyErr_Occurred()) throw pybind11::error_already_set();
+    if (!st || !PyDict_Check(st)) return false;
+    PyObject* so = PyDict_GetItem(st, k_step);
+    PyObject* mo = PyDict_GetItem(st, k_m);
+    PyObject* vo = PyDict_GetItem(st, k_v);
+    if (!so || !mo || !vo || !THPVariable_Check(so) ||
+        !THPVariable_Check(mo) || !THPVariable_Check(vo))
+      return false;
+    const at::Tensor &step = THPVariable_Unpack(so),
+                     &m = THPVariable_Unpack(mo), &v = THPVariable_Unpack(vo);
+    if (!step.is_cpu() || step.scalar_type() != at::kFloat ||
+        step.numel() != 1 || !p.is_cuda() ||
+        (!l.ps.empty() && p.device() != l.ps[0].device()) ||
+        !p.is_non_overlapping_and_dense())
+      return false;
+    for (const at::Tensor* t : {&g, &m, &v})
+      if (t->device() != p.device() || t->scalar_type() != p.scalar_type() ||
+          t->layout() != at::kStrided || t->sizes() != p.sizes() ||
+          (p.numel() > 1 && t->strides() != p.strides()))
+        return false;
+    l.ps.push_back(p);
+    l.gs.push_back(g);
+    l.ms.push_back(m);
+    l.vs.push_back(v);
+    l.steps.push_back(step);
+  }
+  return true;
+}
+
+// kind: 0 Adam, 1 AdamW, 2 LAMB. Returns false, with nothing changed, where
+// read_adam_group does.
+bool fused_adam_group(pybind11::object params, pybind11::object state,
+                      int64_t kind, double lr, double beta1, double beta2,
+                      double eps, double wd,
+                      c10::optional<at::Tensor> grad_scale) {
+  AdamLists l;
+  if (!read_adam_group(params.ptr(), state.ptr(), l)) return false;
+  // One launch for each type and step count, in the order of the parameters.
+  std::vector<std::pair<at::ScalarType, float>> keys;
+  std::vector<AdamLists> parts;
+  for (size_t i = 0; i < l.ps.size(); ++i) {
+    float& step = *l.steps[i].data_ptr<float>();
+    step += 1.0f;
+    const std::pair<at::ScalarType, float> key(l.ps[i].scalar_type(), step);
+    const size_t at = std::find(keys.begin(), keys.end(), key) - keys.begin();
+    if (at == keys.size()) {
+      keys.push_back(key);
+      parts.emplace_back();
+    }
+    AdamLists& part = parts[at];
+    part.ps.push_back(std::move(l.ps[i]));
+    part.gs.push_back(std::move(l.gs[i]));
+    part.ms.push_back(std::move(l.ms[i]));
+    part.vs.push_back(std::move(l.vs[i]));
+  }
+  for (size_t k = 0; k < parts.size(); ++k) {
+    AdamLists& part = parts[k];
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(
+        part.ps[0].device());
+    const int64_t step = static_cast<int64_t>(keys[k].second);
+    if (kind == 2)
+      fused_lamb(std::move(part.ps), std::move(part.gs), std::move(part.ms),
+                 std::move(part.vs), lr, beta1, beta2, eps, wd, step,
+                 grad_scale);
+    else
+      fused_adam(std::move(part.ps), std::move(part.gs), std::move(part.ms),
+                 std::move(part.vs), lr, beta1, beta2, eps, wd, step,
+                 kind == 1, grad_scale);
+  }
+  return true;
+}
+
 }  // namespace
 
 void register_optim(pybind11::module_& m) {
+  m.def("fused_adam_group", &fused_adam_group, pybind11::arg("params"),
+        pybind11::arg("state"), pybind11::arg("kind"), pybind11::arg("lr"),
+        pybind11::arg("beta1"), pybind11::arg("beta2"), pybind11::arg("eps"),
+        pybind11::arg("weight_decay"),
+        pybind11::arg("grad_scale") = pybind11::none());
   m.def("fused_sgd", &fused_sgd, pybind11::arg("params"), pybind11::arg("grads"),
         pybind11::arg("momentum_buffers"), pybind11::arg("lr"),
         pybind11::arg("momentum"), pybind11::arg("dampening"),

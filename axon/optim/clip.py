@@ -98,21 +98,25 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0,
     or give the fused optimizer max_grad_norm, and step() does both.
     """
     norm_type, max_norm = _checked_type(norm_type), _checked_max(max_norm)
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
+    parameters = ([parameters] if isinstance(parameters, torch.Tensor)
+                  else list(parameters))
+    if not error_if_nonfinite:
+        from axon import _core
+
+        out = _core.param_grad_norm([parameters], _TYPES[norm_type], max_norm,
+                                    True)
+        if out is None:
+            return torch.tensor(0.0)
+        if out is not False:
+            return out[0]
     grads = [g for g in (p.grad for p in parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    fast = _fast_path(grads)
-    if fast and not error_if_nonfinite:
-        from axon import _core
-
-        return _core.grad_clip_(grads, _TYPES[norm_type], max_norm)[0]
     norm, factor = norm_and_factor(grads, max_norm, norm_type)
     if error_if_nonfinite and not torch.isfinite(norm):
         raise RuntimeError(f"the norm of order {norm_type} over all gradients "
                            f"is {float(norm)}; the gradients are unchanged")
-    if fast:
+    if _fast_path(grads):
         from axon import _core
 
         _core.grad_scale_(grads, factor)

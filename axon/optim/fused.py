@@ -49,11 +49,19 @@ class _Clipping(Optimizer):
         """The factor for this step, or None."""
         if self.max_grad_norm is None:
             return None
-        grads = [p.grad for group in self.param_groups
-                 for p in group["params"] if p.grad is not None]
-        if not grads:
+        from axon import _core
+
+        out = _core.param_grad_norm(
+            [group["params"] for group in self.param_groups], 2,
+            self.max_grad_norm, False)
+        if out is None:  # no gradients
             return None
-        self.grad_norm, factor = norm_and_factor(grads, self.max_grad_norm)
+        if out is not False:
+            self.grad_norm, factor = out[0], out[1]
+            return factor
+        self.grad_norm, factor = norm_and_factor(
+            [p.grad for group in self.param_groups for p in group["params"]
+             if p.grad is not None], self.max_grad_norm)
         return factor.float()
 
 
@@ -176,6 +184,14 @@ class _FusedAdamBase(_Clipping):
 
         factor = self._clip_factor()
         for group in self.param_groups:
+            b1, b2 = group["betas"]
+            # The steady state, in one call; False (and nothing done) where
+            # state has to be made or mended first, or is not on the GPU.
+            if _core.fused_adam_group(group["params"], self.state,
+                                      1 if self._adamw else 0, group["lr"],
+                                      b1, b2, group["eps"],
+                                      group["weight_decay"], factor):
+                continue
             work = []
             for p in group["params"]:
                 if p.grad is None:
@@ -190,7 +206,6 @@ class _FusedAdamBase(_Clipping):
                 st["exp_avg_sq"] = _like_param(p, st["exp_avg_sq"])
                 work.append((p, _like_param(p, p.grad), st["exp_avg"],
                              st["exp_avg_sq"], int(st["step"].item())))
-            b1, b2 = group["betas"]
             for tuples in _grouped(work):
                 # all params in a (device,dtype) bucket share the step count
                 # only if they were created together; split by step to be safe
@@ -268,6 +283,11 @@ class FusedLAMB(_Clipping):
 
         factor = self._clip_factor()
         for group in self.param_groups:
+            b1, b2 = group["betas"]
+            if _core.fused_adam_group(group["params"], self.state, 2,
+                                      group["lr"], b1, b2, group["eps"],
+                                      group["weight_decay"], factor):
+                continue
             work = []
             for p in group["params"]:
                 if p.grad is None:
@@ -282,7 +302,6 @@ class FusedLAMB(_Clipping):
                 st["exp_avg_sq"] = _like_param(p, st["exp_avg_sq"])
                 work.append((p, _like_param(p, p.grad), st["exp_avg"],
                              st["exp_avg_sq"], int(st["step"].item())))
-            b1, b2 = group["betas"]
             for tuples in _grouped(work):
                 by_step = {}
                 for t in tuples:
