@@ -106,12 +106,27 @@ __global__ void sgd_kernel(const OptChunk* __restrict__ chunks, float lr,
 
 // ---------------------------------------------------------------- Adam(W)
 
+// Chunks of 256K values make few blocks for a large model (5716 for 1.5G
+// values, 2.8 times what runs at once, the last 0.8 of it on a part of the
+// CUs): a chunk is shared by kAdamParts blocks. 1.5G bf16 values: 4963 us with
+// one block for each chunk, 4594 with 4, 4525 with 8.
+constexpr int kAdamParts = 8;
+constexpr int64_t kAlign = 8;  // parts start on vectors
+
 template <typename T>
 __global__ void adam_kernel(const OptChunk* __restrict__ chunks, float lr,
                             float beta1, float beta2, float eps, float wd,
                             float bc1, float bc2_sqrt, int adamw,
                             const float* __restrict__ gscale) {
-  const OptChunk c = chunks[blockIdx.x];
+  // The chunk's part of this block.
+  OptChunk c = chunks[blockIdx.x];
+  const int64_t part = c.n / kAlign / gridDim.y * kAlign;
+  const int64_t from = part * blockIdx.y;
+  c.p = static_cast<T*>(c.p) + from;
+  c.g = static_cast<T*>(c.g) + from;
+  c.m = static_cast<T*>(c.m) + from;
+  c.v = static_cast<T*>(c.v) + from;
+  c.n = blockIdx.y + 1 == gridDim.y ? c.n - from : part;
   T* __restrict__ p = static_cast<T*>(c.p);
   const T* __restrict__ g = static_cast<const T*>(c.g);
   T* __restrict__ m = static_cast<T*>(c.m);
@@ -293,7 +308,7 @@ void launch_fused_adam(const OptChunk* chunks, int nchunks, int dtype, float lr,
                        float bc2_sqrt, bool adamw, const float* gscale,
                        hipStream_t stream) {
   if (nchunks <= 0) return;
-  dim3 grid(nchunks), block(kThreads);
+  dim3 grid(nchunks, kAdamParts), block(kThreads);
   DISPATCH(adam_kernel, chunks, lr, beta1, beta2, eps, wd, bc1, bc2_sqrt,
            adamw ? 1 : 0, gscale);
 }
