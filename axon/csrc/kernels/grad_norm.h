@@ -32,5 +32,11 @@ void launch_grad_finish(const double* partial, int blocks, int type,
 // g *= *factor; nothing is read or written where *factor is 1.
 void launch_grad_scale(const GradTable& t, int dtype, const float* factor,
                        hipStream_t stream);
+// Both in one launch for each table, where all partial sums are few (each
+// block joins them): out as above, written by each of the launches alike.
+bool grad_clip_folds(int blocks);
+void launch_grad_clip(const GradTable& t, int dtype, int type,
+                      const double* partial, int blocks, float max_norm,
+                      float* out, hipStream_t stream);
 
 }  // namespace axon

@@ -105,29 +105,46 @@ __global__ __launch_bounds__(kThreads) void grad_partial_kernel(
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
+// (norm, factor) of the partial sums, in every thread of the block, and the
+// same bits in every block.
 template <int kType>
-__global__ __launch_bounds__(kThreads) void grad_finish_kernel(
-    const double* __restrict__ partial, int blocks, float max_norm,
-    float* __restrict__ out) {
+__device__ __forceinline__ float2 finish(const double* __restrict__ partial,
+                                         int blocks, float max_norm) {
   using J = std::conditional_t<kType == 0, Most, Sum>;
   double acc = 0.0;
   for (int i = threadIdx.x; i < blocks; i += kThreads)
     acc = J::join(acc, partial[i]);
   acc = block_join<J>(acc);
-  if (threadIdx.x == 0) {
-    const float norm = static_cast<float>(kType == 2 ? sqrt(acc) : acc);
-    const float c = max_norm / (norm + 1e-6f);
-    out[0] = norm;
-    out[1] = c > 1.f ? 1.f : c;  // NaN stays
-  }
+  const float norm = static_cast<float>(kType == 2 ? sqrt(acc) : acc);
+  const float c = max_norm / (norm + 1e-6f);
+  return make_float2(norm, c > 1.f ? 1.f : c);  // NaN stays
 }
 
-template <typename T>
+template <int kType>
+__global__ __launch_bounds__(kThreads) void grad_finish_kernel(
+    const double* __restrict__ partial, int blocks, float max_norm,
+    float2* __restrict__ out) {
+  const float2 r = finish<kType>(partial, blocks, max_norm);
+  if (threadIdx.x == 0) *out = r;
+}
+
+// kType >= 0: every block joins the (few) partial sums itself, and the first
+// one writes the result; kType < 0: the factor is there.
+template <typename T, int kType>
 __global__ __launch_bounds__(kThreads) void grad_scale_kernel(
-    const GradTable t, const float* __restrict__ factor) {
+    const GradTable t, const float* __restrict__ factor,
+    const double* __restrict__ partial, int blocks, float max_norm,
+    float2* __restrict__ out) {
   constexpr int V = kVec<T>;
   constexpr int kAhead = 4;
-  const float c = *factor;
+  float c;
+  if constexpr (kType < 0) {
+    c = *factor;
+  } else {
+    const float2 r = finish<kType>(partial, blocks, max_norm);
+    c = r.y;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *out = r;
+  }
   if (c == 1.f) return;
   const int chunks = t.first[t.count];
   for (int b = blockIdx.x; b < chunks; b += gridDim.x) {
@@ -191,16 +208,41 @@ void launch_grad_finish(const double* partial, int blocks, int type,
             : type == 1 ? grad_finish_kernel<1>
                         : grad_finish_kernel<0>;
   hipLaunchKernelGGL(k, dim3(1), dim3(kThreads), 0, stream, partial, blocks,
-                     max_norm, out);
+                     max_norm, reinterpret_cast<float2*>(out));
 }
+
+namespace {
+
+template <int kType>
+void scale(const GradTable& t, int dtype, const float* factor,
+           const double* partial, int blocks, float max_norm, float* out,
+           hipStream_t stream) {
+  auto* k = dtype == kFloat  ? grad_scale_kernel<float, kType>
+            : dtype == kHalf ? grad_scale_kernel<_Float16, kType>
+                             : grad_scale_kernel<__bf16, kType>;
+  hipLaunchKernelGGL(k, dim3(grad_norm_blocks(t)), dim3(kThreads), 0, stream, t,
+                     factor, partial, blocks, max_norm,
+                     reinterpret_cast<float2*>(out));
+}
+
+}  // namespace
 
 void launch_grad_scale(const GradTable& t, int dtype, const float* factor,
                        hipStream_t stream) {
-  auto* k = dtype == kFloat  ? grad_scale_kernel<float>
-            : dtype == kHalf ? grad_scale_kernel<_Float16>
-                             : grad_scale_kernel<__bf16>;
-  hipLaunchKernelGGL(k, dim3(std::min(kMaxBlocks, t.first[t.count])),
-                     dim3(kThreads), 0, stream, t, factor);
+  scale<-1>(t, dtype, factor, nullptr, 0, 0.f, nullptr, stream);
+}
+
+bool grad_clip_folds(int blocks) { return blocks <= 2 * kThreads; }
+
+void launch_grad_clip(const GradTable& t, int dtype, int type,
+                      const double* partial, int blocks, float max_norm,
+                      float* out, hipStream_t stream) {
+  if (type == 2)
+    scale<2>(t, dtype, nullptr, partial, blocks, max_norm, out, stream);
+  if (type == 1)
+    scale<1>(t, dtype, nullptr, partial, blocks, max_norm, out, stream);
+  if (type == 0)
+    scale<0>(t, dtype, nullptr, partial, blocks, max_norm, out, stream);
 }
 
 }  // namespace axon

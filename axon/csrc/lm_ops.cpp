@@ -75,14 +75,15 @@ at::Tensor embed_bwd(const at::Tensor& ids, const at::Tensor& dy_in,
       at::empty({(vocab * dim + unit - 1) / unit * unit}, dy.options());
   if (dw.numel() == 0) return dw.view({vocab, dim});
   dw = dw.as_strided({vocab, dim}, {dim, 1});
-  at::Tensor keys = at::empty({2 * n}, ids.options().dtype(at::kLong));
-  at::Tensor part =
-      at::empty({embed_part_floats(n, dim, static_cast<int>(dy.element_size()))},
-                dy.options().dtype(at::kFloat));
+  // Keys, twice, and partial sums.
+  const int64_t parts =
+      embed_part_floats(n, dim, static_cast<int>(dy.element_size()));
+  at::Tensor scratch =
+      at::empty({4 * n + parts}, dy.options().dtype(at::kFloat));
+  float* const part = scratch.data_ptr<float>() + 4 * n;
   launch_embed_bwd(code_of(dy), ids.scalar_type() == at::kLong, ids.data_ptr(),
                    dy.data_ptr(), dw.data_ptr(),
-                   reinterpret_cast<uint64_t*>(keys.data_ptr()),
-                   part.data_ptr<float>(), n, vocab, dim, padding,
+                   reinterpret_cast<uint64_t*>(scratch.data_ptr()), part, n, vocab, dim, padding,
                    static_cast<float>(scale), stream_of(dy));
   check_launch();
   return dw;
@@ -191,7 +192,8 @@ LogitRows logit_rows(const at::Tensor& x, const at::Tensor& target) {
 
 struct CrossEntropyBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable logits, target;
-  at::Tensor kept, factor;  // of this file alone
+  at::Tensor kept;  // of this file alone: from kept_at on
+  int64_t kept_at = 0;
   int64_t ignore = 0;
   double eps = 0.0;
   int reduction = 1;
@@ -211,13 +213,13 @@ struct CrossEntropyBackward : public torch::autograd::Node {
                       g.numel() == (reduction == 0 ? r.n : 1),
                   "cross_entropy: the loss's gradient");
       dx = at::empty(x.sizes(), x.options());
+      const float* const k = kept.data_ptr<float>() + kept_at;
       if (r.n > 0) {
         launch_ce_bwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
                       r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n,
                       r.vocab, static_cast<float>(eps),
-                      kept.data_ptr<float>(), g.data_ptr<float>(),
-                      reduction == 0 ? 1 : 0,
-                      reduction == 0 ? nullptr : factor.data_ptr<float>(),
+                      k, g.data_ptr<float>(), reduction == 0 ? 1 : 0,
+                      reduction == 0 ? nullptr : k + 2 * r.n,
                       dx.data_ptr(), stream_of(x));
         check_launch();
       }
@@ -229,7 +231,6 @@ struct CrossEntropyBackward : public torch::autograd::Node {
     logits.reset_data();
     target.reset_data();
     kept.reset();
-    factor.reset();
   }
   std::string name() const override { return "AxonCrossEntropyBackward"; }
 };
@@ -294,19 +295,19 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
     // The loss, which its user may change in place, is memory of its own.
     loss = reduction == 0 ? at::empty(target.sizes(), fopt)
                           : at::empty({}, fopt);
-    at::Tensor kept = at::empty({2 * r.n + 1}, fopt);
-    at::Tensor factor = kept.narrow(0, 2 * r.n, 1);
-    at::Tensor scratch = at::empty({ce_scratch_bytes(r.n, r.vocab)},
-                                   x.options().dtype(at::kByte));
+    // Scratch (whole doubles), and what the backward pass takes: a row's
+    // (m, 1/S), and the factor at its end.
+    const int64_t scratch = (ce_scratch_bytes(r.n, r.vocab) + 7) / 8 * 2;
+    at::Tensor work = at::empty({scratch + 2 * r.n + 1}, fopt);
+    float* const kept = work.data_ptr<float>() + scratch;
     launch_ce_fwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
                   r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n, r.vocab,
-                  static_cast<float>(eps), reduction, scratch.data_ptr(),
-                  kept.data_ptr<float>(), loss.data_ptr<float>(),
-                  factor.data_ptr<float>(), stream_of(x));
+                  static_cast<float>(eps), reduction, work.data_ptr(), kept,
+                  loss.data_ptr<float>(), kept + 2 * r.n, stream_of(x));
     check_launch();
     if (node) {
-      node->kept = kept;
-      node->factor = factor;
+      node->kept = work;
+      node->kept_at = scratch;
     }
   }
   if (node) torch::autograd::set_history(loss, node);
@@ -403,29 +404,6 @@ void for_tables(const std::vector<at::Tensor>& ts, F f) {
   }
 }
 
-at::Tensor norm_of(const Grads& g, const at::Tensor& like, int64_t type,
-                   double max_norm) {
-  const auto opt = like.options();
-  at::Tensor out = at::empty({2}, opt.dtype(at::kFloat));
-  int blocks = 0;
-  for_tables(g.dense, [&](const GradTable& t, int) {
-    blocks += grad_norm_blocks(t);
-  });
-  at::Tensor partial = at::empty({blocks}, opt.dtype(at::kDouble));
-  const hipStream_t stream = stream_of(like);
-  int at = 0;
-  for_tables(g.dense, [&](const GradTable& t, int dtype) {
-    launch_grad_partial(t, dtype, static_cast<int>(type),
-                        partial.data_ptr<double>() + at, stream);
-    at += grad_norm_blocks(t);
-  });
-  launch_grad_finish(partial.data_ptr<double>(), blocks,
-                     static_cast<int>(type), static_cast<float>(max_norm),
-                     out.data_ptr<float>(), stream);
-  check_launch();
-  return out;
-}
-
 void scale_by(const Grads& g, const at::Tensor& like, const float* factor) {
   const hipStream_t stream = stream_of(like);
   for_tables(g.dense, [&](const GradTable& t, int dtype) {
@@ -435,23 +413,48 @@ void scale_by(const Grads& g, const at::Tensor& like, const float* factor) {
   for (auto& s : g.strided) s.first.copy_(g.dense[s.second]);
 }
 
-// (norm, factor) as fp32[2]; type 0 is the maximum.
-at::Tensor grad_norm(const std::vector<at::Tensor>& ts, int64_t type,
-                     double max_norm) {
+// (norm, factor) as fp32[2], and the tensors scaled by the factor if `clip`;
+// type 0 is the maximum.
+at::Tensor norm_of(const std::vector<at::Tensor>& ts, int64_t type,
+                   double max_norm, bool clip) {
   TORCH_CHECK(type >= 0 && type <= 2, "grad norm: type");
-  const Grads g = collect(ts, false);
+  const Grads g = collect(ts, clip);
   const Guard guard(ts[0].device());
-  return norm_of(g, ts[0], type, max_norm);
+  const auto opt = ts[0].options();
+  int blocks = 0;
+  for_tables(g.dense, [&](const GradTable& t, int) {
+    blocks += grad_norm_blocks(t);
+  });
+  at::Tensor out = at::empty({2}, opt.dtype(at::kFloat));
+  at::Tensor partial = at::empty({blocks}, opt.dtype(at::kDouble));
+  const hipStream_t stream = stream_of(ts[0]);
+  const int kind = static_cast<int>(type);
+  double* const sums = partial.data_ptr<double>();
+  float* const result = out.data_ptr<float>();
+  int at = 0;
+  for_tables(g.dense, [&](const GradTable& t, int dtype) {
+    launch_grad_partial(t, dtype, kind, sums + at, stream);
+    at += grad_norm_blocks(t);
+  });
+  if (clip && blocks > 0 && grad_clip_folds(blocks)) {
+    for_tables(g.dense, [&](const GradTable& t, int dtype) {
+      launch_grad_clip(t, dtype, kind, sums, blocks,
+                       static_cast<float>(max_norm), result, stream);
+    });
+    check_launch();
+    for (auto& s : g.strided) s.first.copy_(g.dense[s.second]);
+    return out;
+  }
+  launch_grad_finish(sums, blocks, kind, static_cast<float>(max_norm), result,
+                     stream);
+  check_launch();
+  if (clip) scale_by(g, ts[0], result + 1);
+  return out;
 }
 
-at::Tensor grad_clip_(const std::vector<at::Tensor>& ts, int64_t type,
-                      double max_norm) {
-  TORCH_CHECK(type >= 0 && type <= 2, "grad norm: type");
-  const Grads g = collect(ts, true);
-  const Guard guard(ts[0].device());
-  at::Tensor out = norm_of(g, ts[0], type, max_norm);
-  scale_by(g, ts[0], out.data_ptr<float>() + 1);
-  return out;
+at::Tensor grad_norm(const std::vector<at::Tensor>& ts, int64_t type,
+                     double max_norm) {
+  return norm_of(ts, type, max_norm, false);
 }
 
 // The gradients of lists of parameters, read here rather than in Python:
@@ -482,8 +485,7 @@ pybind11::object param_grad_norm(const pybind11::list& lists, int64_t type,
   std::vector<at::Tensor> grads;
   if (!param_grads(lists, grads)) return pybind11::bool_(false);
   if (grads.empty()) return pybind11::none();
-  return pybind11::cast(clip ? grad_clip_(grads, type, max_norm)
-                             : grad_norm(grads, type, max_norm));
+  return pybind11::cast(norm_of(grads, type, max_norm, clip));
 }
 
 void grad_scale_(const std::vector<at::Tensor>& ts, const at::Tensor& factor) {
