@@ -161,7 +161,14 @@ __global__ __launch_bounds__(kThreads) void ce_stat_kernel(
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) take(r[k]);
       }
-      for (; i < full; i += G) take(load<kOnce>(body + i * V));
+      // Up to three are left: loaded together as well.
+      u32x4 r[kAhead - 1];
+#pragma unroll
+      for (int k = 0; k < kAhead - 1; ++k)
+        if (i + k * G < full) r[k] = load<kOnce>(body + (i + k * G) * V);
+#pragma unroll
+      for (int k = 0; k < kAhead - 1; ++k)
+        if (i + k * G < full) take(r[k]);
     };
     if (row < once_rows)
       vectors(std::true_type{});
@@ -343,7 +350,13 @@ __global__ __launch_bounds__(kThreads) void ce_grad_kernel(
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) put(r[k], i + k * G);
     }
-    for (; i < full; i += G) put(load<kReadOnce>(body + i * V), i);
+    u32x4 r[kAhead - 1];
+#pragma unroll
+    for (int k = 0; k < kAhead - 1; ++k)
+      if (i + k * G < full) r[k] = load<kReadOnce>(body + (i + k * G) * V);
+#pragma unroll
+    for (int k = 0; k < kAhead - 1; ++k)
+      if (i + k * G < full) put(r[k], i + k * G);
   };
   for (int j = t; j < head; j += G) one(j);
   if (kOnce && row < once_rows)

@@ -147,7 +147,10 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(
   }
   if (c == 1.f) return;
   const int chunks = t.first[t.count];
-  for (int b = blockIdx.x; b < chunks; b += gridDim.x) {
+  // From the last chunk to the first: the norm has just read the last ones,
+  // and the chip's last cache holds 256 MB of them.
+  for (int b = chunks - 1 - static_cast<int>(blockIdx.x); b >= 0;
+       b -= gridDim.x) {
     const int i = tensor_of(t, b);
     const int64_t begin = static_cast<int64_t>(b - t.first[i]) * kGradChunk;
     T* p = static_cast<T*>(t.ptr[i]) + begin;

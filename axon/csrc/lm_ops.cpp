@@ -376,40 +376,38 @@ Grads collect(const std::vector<at::Tensor>& ts, bool written) {
   return g;
 }
 
-// Calls f(table, dtype) for tables that cover all tensors, one type each.
-template <typename F>
-void for_tables(const std::vector<at::Tensor>& ts, F f) {
+struct Table {
+  GradTable t;
+  int dtype;
+};
+
+// Tables that cover all tensors, one type each.
+std::vector<Table> tables_of(const std::vector<at::Tensor>& ts) {
+  std::vector<Table> tables;
   for (auto type : {at::kFloat, at::kHalf, at::kBFloat16}) {
-    GradTable t;
-    t.count = 0;
-    t.first[0] = 0;
-    auto done = [&] {
-      if (t.count) f(t, static_cast<int>(type));
-      t.count = 0;
-    };
+    GradTable* t = nullptr;
     for (const at::Tensor& x : ts) {
       if (x.scalar_type() != type) continue;
       const int64_t chunks = (x.numel() + kGradChunk - 1) / kGradChunk;
       TORCH_CHECK(chunks < (int64_t{1} << 30), "grad norm: tensor too large");
-      if (t.count == kGradTensors ||
-          (t.count && t.first[t.count] + chunks >= (int64_t{1} << 30)))
-        done();
-      t.ptr[t.count] = x.data_ptr();
-      t.n[t.count] = x.numel();
-      t.first[t.count + 1] =
-          t.first[t.count] + static_cast<int32_t>(chunks);
-      ++t.count;
+      if (!t || t->count == kGradTensors ||
+          t->first[t->count] + chunks >= (int64_t{1} << 30)) {
+        tables.emplace_back();
+        tables.back().dtype = static_cast<int>(type);
+        t = &tables.back().t;
+        t->count = 0;
+        t->first[0] = 0;
+      }
+      t->ptr[t->count] = x.data_ptr();
+      t->n[t->count] = x.numel();
+      t->first[t->count + 1] = t->first[t->count] + static_cast<int32_t>(chunks);
+      ++t->count;
     }
-    done();
   }
+  return tables;
 }
 
-void scale_by(const Grads& g, const at::Tensor& like, const float* factor) {
-  const hipStream_t stream = stream_of(like);
-  for_tables(g.dense, [&](const GradTable& t, int dtype) {
-    launch_grad_scale(t, dtype, factor, stream);
-  });
-  check_launch();
+void write_back(const Grads& g) {
   for (auto& s : g.strided) s.first.copy_(g.dense[s.second]);
 }
 
@@ -421,34 +419,35 @@ at::Tensor norm_of(const std::vector<at::Tensor>& ts, int64_t type,
   const Grads g = collect(ts, clip);
   const Guard guard(ts[0].device());
   const auto opt = ts[0].options();
+  const std::vector<Table> tables = tables_of(g.dense);
   int blocks = 0;
-  for_tables(g.dense, [&](const GradTable& t, int) {
-    blocks += grad_norm_blocks(t);
-  });
+  for (const Table& t : tables) blocks += grad_norm_blocks(t.t);
   at::Tensor out = at::empty({2}, opt.dtype(at::kFloat));
   at::Tensor partial = at::empty({blocks}, opt.dtype(at::kDouble));
   const hipStream_t stream = stream_of(ts[0]);
   const int kind = static_cast<int>(type);
+  const float bound = static_cast<float>(max_norm);
   double* const sums = partial.data_ptr<double>();
   float* const result = out.data_ptr<float>();
   int at = 0;
-  for_tables(g.dense, [&](const GradTable& t, int dtype) {
-    launch_grad_partial(t, dtype, kind, sums + at, stream);
-    at += grad_norm_blocks(t);
-  });
-  if (clip && blocks > 0 && grad_clip_folds(blocks)) {
-    for_tables(g.dense, [&](const GradTable& t, int dtype) {
-      launch_grad_clip(t, dtype, kind, sums, blocks,
-                       static_cast<float>(max_norm), result, stream);
-    });
-    check_launch();
-    for (auto& s : g.strided) s.first.copy_(g.dense[s.second]);
-    return out;
+  for (const Table& t : tables) {
+    launch_grad_partial(t.t, t.dtype, kind, sums + at, stream);
+    at += grad_norm_blocks(t.t);
   }
-  launch_grad_finish(sums, blocks, kind, static_cast<float>(max_norm), result,
-                     stream);
+  const bool folds = clip && blocks > 0 && grad_clip_folds(blocks);
+  if (!folds) launch_grad_finish(sums, blocks, kind, bound, result, stream);
+  if (clip) {
+    // What the norm read last comes first.
+    for (auto t = tables.rbegin(); t != tables.rend(); ++t) {
+      if (folds)
+        launch_grad_clip(t->t, t->dtype, kind, sums, blocks, bound, result,
+                         stream);
+      else
+        launch_grad_scale(t->t, t->dtype, result + 1, stream);
+    }
+    write_back(g);
+  }
   check_launch();
-  if (clip) scale_by(g, ts[0], result + 1);
   return out;
 }
 
@@ -494,7 +493,11 @@ void grad_scale_(const std::vector<at::Tensor>& ts, const at::Tensor& factor) {
                   factor.scalar_type() == at::kFloat,
               "grad scale: the factor must be one float on the tensors' GPU");
   const Guard guard(ts[0].device());
-  scale_by(g, ts[0], factor.data_ptr<float>());
+  for (const Table& t : tables_of(g.dense))
+    launch_grad_scale(t.t, t.dtype, factor.data_ptr<float>(),
+                      stream_of(ts[0]));
+  write_back(g);
+  check_launch();
 }
 
 }  // namespace
