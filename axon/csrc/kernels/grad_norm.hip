@@ -40,15 +40,15 @@ __device__ __forceinline__ double add(double acc, float f) {
   return Most::join(acc, fabs(d));
 }
 
-template <typename J>
+template <typename J, int kBlock = kThreads>
 __device__ double block_join(double v) {
-  __shared__ double lds[kThreads / 64];
+  __shared__ double lds[kBlock / 64];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v = J::join(v, __shfl_xor(v, off, 64));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   v = lds[0];
-  for (int w = 1; w < kThreads / 64; ++w) v = J::join(v, lds[w]);
+  for (int w = 1; w < kBlock / 64; ++w) v = J::join(v, lds[w]);
   return v;
 }
 
@@ -107,24 +107,26 @@ __global__ __launch_bounds__(kThreads) void grad_partial_kernel(
 
 // (norm, factor) of the partial sums, in every thread of the block, and the
 // same bits in every block.
-template <int kType>
+template <int kType, int kBlock = kThreads>
 __device__ __forceinline__ float2 finish(const double* __restrict__ partial,
                                          int blocks, float max_norm) {
   using J = std::conditional_t<kType == 0, Most, Sum>;
   double acc = 0.0;
-  for (int i = threadIdx.x; i < blocks; i += kThreads)
+  for (int i = threadIdx.x; i < blocks; i += kBlock)
     acc = J::join(acc, partial[i]);
-  acc = block_join<J>(acc);
+  acc = block_join<J, kBlock>(acc);
   const float norm = static_cast<float>(kType == 2 ? sqrt(acc) : acc);
   const float c = max_norm / (norm + 1e-6f);
   return make_float2(norm, c > 1.f ? 1.f : c);  // NaN stays
 }
 
+constexpr int kFinishThreads = 1024;
+
 template <int kType>
-__global__ __launch_bounds__(kThreads) void grad_finish_kernel(
+__global__ __launch_bounds__(kFinishThreads) void grad_finish_kernel(
     const double* __restrict__ partial, int blocks, float max_norm,
     float2* __restrict__ out) {
-  const float2 r = finish<kType>(partial, blocks, max_norm);
+  const float2 r = finish<kType, kFinishThreads>(partial, blocks, max_norm);
   if (threadIdx.x == 0) *out = r;
 }
 
@@ -210,7 +212,7 @@ void launch_grad_finish(const double* partial, int blocks, int type,
   auto* k = type == 2   ? grad_finish_kernel<2>
             : type == 1 ? grad_finish_kernel<1>
                         : grad_finish_kernel<0>;
-  hipLaunchKernelGGL(k, dim3(1), dim3(kThreads), 0, stream, partial, blocks,
+  hipLaunchKernelGGL(k, dim3(1), dim3(kFinishThreads), 0, stream, partial, blocks,
                      max_norm, reinterpret_cast<float2*>(out));
 }
 
