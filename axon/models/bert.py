@@ -83,8 +83,8 @@ class BertForPreTraining(nn.Module):
         super().__init__()
         self.cfg = cfg
         self.tok = FusedEmbedding(cfg.vocab_size, cfg.hidden)
-        self.pos = nn.Embedding(cfg.max_seq, cfg.hidden)
-        self.typ = nn.Embedding(cfg.type_vocab, cfg.hidden)
+        self.pos = FusedEmbedding(cfg.max_seq, cfg.hidden)
+        self.typ = FusedEmbedding(cfg.type_vocab, cfg.hidden)
         self.ln_emb = FusedLayerNorm(cfg.hidden)
         self.layers = nn.ModuleList(BertLayer(cfg) for _ in range(cfg.layers))
         self.mlm_dense = nn.Linear(cfg.hidden, cfg.hidden)

@@ -745,6 +745,203 @@ def test_refusals_gpu():
         g.sum().backward()
 
 
+def test_large_logits():
+    """Logits of more than the caches' share (both kinds of rows in one
+    call), and rows that do not start on lines."""
+    for n, vocab, dtype in [(3500, 30522, torch.bfloat16),
+                            (900, 60001, torch.float32)]:
+        x, t, g = _logits(n, vocab, dtype)
+        t[torch.rand(n, generator=g, device=DEV) < 0.5] = -100
+        _loss_check(x, t)
+        del x
+        torch.cuda.empty_cache()
+
+
+def test_many_rows():
+    """More rows than one block sums."""
+    for n, vocab in [(16384, 5), (16385, 40), (200001, 3)]:
+        x, t, g = _logits(n, vocab, torch.float32)
+        t[torch.rand(n, generator=g, device=DEV) < 0.2] = -100
+        _loss_check(x, t)
+
+
+def test_clip_many_blocks():
+    """More partial sums than the scaling blocks join themselves, more
+    chunks than blocks, two types."""
+    _clip_check(_params([(12_000_001,), (7,), (36_000_000,)],
+                        [torch.float32, torch.float32, torch.bfloat16]), 1.0)
+    _clip_check(_params([(20_000_000,)], [torch.float16], std=0.01), 2.0, 1.0)
+
+
+def test_no_gradient_modes():
+    from axon.ops import cross_entropy, embedding
+
+    w = torch.randn(20, 16, device=DEV, requires_grad=True)
+    ids = torch.arange(12, device=DEV)
+    with torch.no_grad():
+        assert not embedding(ids, w).requires_grad
+        assert not cross_entropy(w, torch.arange(20, device=DEV) % 16
+                                 ).requires_grad
+    with torch.inference_mode():
+        x = torch.randn(12, 16, device=DEV)
+        assert torch.isfinite(cross_entropy(x, ids))
+        assert torch.equal(embedding(ids, x), x)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = cross_entropy(w @ w.t(), torch.arange(20, device=DEV))
+    assert loss.dtype == torch.float32
+    loss.backward()
+    assert torch.isfinite(w.grad).all()
+
+
+def test_graph_is_freed_and_guarded():
+    """Twice backward, an input changed in between, forward-mode."""
+    import torch.autograd.forward_ad as fwad
+
+    from axon.ops import cross_entropy, embedding
+
+    x = torch.randn(6, 9, device=DEV, requires_grad=True)
+    t = torch.arange(6, device=DEV)
+    loss = cross_entropy(x, t)
+    loss.backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
+    y = embedding(t, x)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    z = x.detach() * 2.0
+    z.requires_grad_()
+    mid = z * 1.0
+    loss = cross_entropy(mid, t)
+    with torch.no_grad():
+        mid.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with fwad.dual_level():
+        dual = fwad.make_dual(x.detach(), torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            cross_entropy(dual, t)
+        with pytest.raises(NotImplementedError):
+            embedding(t, dual)
+
+
+def test_threads():
+    """Calls from two threads, each on a stream of its own."""
+    import threading
+
+    from axon.ops import cross_entropy, embedding
+    from axon.optim import grad_norm
+
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(300, 3000, generator=g, device=DEV)
+    t = torch.randint(3000, (300,), generator=g, device=DEV)
+    ids = torch.randint(300, (4000,), generator=g, device=DEV)
+    dy = torch.randn(4000, 3000, generator=g, device=DEV)
+
+    def work():
+        leaf = x.clone().requires_grad_()
+        loss = cross_entropy(leaf, t)
+        (a,) = torch.autograd.grad(loss, leaf)
+        (b,) = torch.autograd.grad(embedding(ids, leaf), leaf, dy)
+        return [loss.detach(), a, b, grad_norm([a, b])]
+
+    want = work()
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def run(name):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    got[name] = work()
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    for r in got.values():
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
+@pytest.mark.parametrize("name", ["Adam", "AdamW", "LAMB"])
+@pytest.mark.parametrize("clip", [None, 0.5])
+def test_group_path_is_the_general_path(name, clip, monkeypatch):
+    """The step that reads a whole group in one call against the one that
+    goes by each parameter: other layouts, types, step counts, parameters
+    without a gradient, state that does not exist yet."""
+    import axon.optim
+    from axon import _core
+
+    def make():
+        ps = _params([(33, 7), (5,), (4, 6, 5, 3), (2000,), (64,)],
+                     [torch.float32, torch.bfloat16, torch.float32,
+                      torch.bfloat16, torch.float32], seed=3)
+        ps[2].data = ps[2].data.to(memory_format=torch.channels_last)
+        g = torch.Generator(device=DEV).manual_seed(8)
+        for p in ps:
+            p.data.normal_(generator=g)
+        return ps, getattr(axon.optim, "Fused" + name)(
+            [{"params": ps[:3]}, {"params": ps[3:], "lr": 0.02}], lr=0.01,
+            weight_decay=0.1, max_grad_norm=clip)
+
+    def steps(ps, opt):
+        g = torch.Generator(device=DEV).manual_seed(1)
+        for i in range(4):
+            for k, p in enumerate(ps):
+                p.grad = torch.randn(p.shape, generator=g,
+                                     device=DEV).to(p.dtype)
+                if k == 2 and i != 1:  # once of another layout than p
+                    p.grad = p.grad.to(memory_format=torch.channels_last)
+            if i < 2:
+                ps[1].grad = None
+            opt.step()
+        return [p.detach() for p in ps] + [
+            v for p in ps for k, v in sorted(opt.state[p].items())]
+
+    calls = []
+    whole = _core.fused_adam_group
+    monkeypatch.setattr(_core, "fused_adam_group",
+                        lambda *a: calls.append(whole(*a)) or calls[-1])
+    got = steps(*make())
+    assert True in calls and False in calls
+    monkeypatch.setattr(_core, "fused_adam_group", lambda *a: False)
+    want = steps(*make())
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and a.stride() == b.stride()
+        if name == "LAMB":
+            # Its norms are added with atomics, in any order: 2000 values'
+            # fp32 sum, then half a step of the type.
+            eps = torch.finfo(a.dtype).eps
+            assert torch.allclose(a.double(), b.double(),
+                                  rtol=max(2000 * U, eps),
+                                  atol=max(1e-6, eps / 100))
+        else:
+            assert torch.equal(a, b)
+
+
+def test_clipping_under_distributed_optimizer():
+    import axon as hvd
+    from axon.optim import FusedAdamW
+
+    hvd.init()
+    try:
+        p = torch.nn.Parameter(torch.zeros(3, device=DEV))
+        opt = hvd.DistributedOptimizer(
+            FusedAdamW([p], lr=0.1, max_grad_norm=1.0),
+            named_parameters=[("p", p)])
+        (p * torch.tensor([6.0, 8.0, 0.0], device=DEV)).sum().backward()
+        opt.step()
+        assert abs(float(opt.grad_norm) - 10.0) <= 10.0 * U
+    finally:
+        hvd.shutdown()
+
+
 def test_models_use_the_kernels():
     """Both language models' losses and gradients on the GPU against the
     same weights through torch's own functions."""
@@ -754,23 +951,27 @@ def test_models_use_the_kernels():
     from axon.models.llama import LlamaForCausalLM, llama_tiny_config
     from axon.ops import FusedEmbedding
 
+    def compare(model, got, want):
+        # Losses over some 100 classes: a few tens of roundings. Gradients of
+        # the vocabulary's table: products of at most 128 values and sums of
+        # 64 rows on both sides, compared by norms.
+        assert abs(got.item() - want.item()) <= 100 * U * want.item()
+        table = (model.embed if hasattr(model, "embed") else model.tok).weight
+        (a,) = torch.autograd.grad(got, table)
+        (b,) = torch.autograd.grad(want, table)
+        assert (a - b).norm() <= 1000 * U * b.norm()
+
     torch.manual_seed(0)
     llama = LlamaForCausalLM(llama_tiny_config()).to(DEV)
     assert isinstance(llama.embed, FusedEmbedding)
     ids = torch.randint(256, (2, 32), device=DEV)
-    logits = llama(ids)
-    want = F.cross_entropy(logits[:, :-1].double().flatten(0, 1),
-                           ids[:, 1:].flatten())
-    got = llama.lm_loss(ids)
-    # 256 classes: a few tens of roundings.
-    assert abs(float(got) - float(want)) <= 100 * U * float(want)
-    got.backward()
-    assert llama.embed.weight.grad.abs().sum() > 0
+    compare(llama, llama.lm_loss(ids),
+            F.cross_entropy(llama(ids)[:, :-1].double().flatten(0, 1),
+                            ids[:, 1:].flatten()))
     bert = BertForPreTraining(bert_tiny_config()).to(DEV)
+    assert isinstance(bert.tok, FusedEmbedding)
     ids = torch.randint(128, (2, 32), device=DEV)
     labels = torch.where(torch.rand(2, 32, device=DEV) < 0.3, ids, -100)
-    want = F.cross_entropy(bert(ids).double().view(-1, 128), labels.view(-1))
-    got = bert.mlm_loss(ids, labels)
-    assert abs(float(got) - float(want)) <= 100 * U * float(want)
-    got.backward()
-    assert bert.tok.weight.grad.abs().sum() > 0
+    compare(bert, bert.mlm_loss(ids, labels),
+            F.cross_entropy(bert(ids).double().view(-1, 128),
+                            labels.view(-1)))
