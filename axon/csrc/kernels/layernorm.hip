@@ -60,7 +60,7 @@ __device__ __forceinline__ float ln_wave_sum(float v) {
 // One WAVE per row, registers only (see the backward below).
 
 template <typename T, int VC, int CH>
-__global__ void ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
+__global__ __launch_bounds__(kThreads) void ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
                               const T* __restrict__ b, T* __restrict__ y,
                               float* __restrict__ mean_out,
                               float* __restrict__ rstd_out, int64_t rows, int H,
@@ -120,7 +120,7 @@ __global__ void ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
 // Two row sums (s1 = sum g, s2 = sum g*xhat) reduce with xor-shuffles.
 
 template <typename T, int VC, int CH>
-__global__ void ln_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+__global__ __launch_bounds__(kThreads) void ln_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dy,
                               const T* __restrict__ w,
                               const float* __restrict__ mean_in,
                               const float* __restrict__ rstd_in,

@@ -78,7 +78,7 @@ __device__ __forceinline__ float rms_wave_sum_f(float v) {
 }
 
 template <typename T, int VC, int CH>
-__global__ void rms_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
+__global__ __launch_bounds__(kThreads) void rms_fwd_kernel(const T* __restrict__ x, const T* __restrict__ w,
                                T* __restrict__ y, float* __restrict__ rstd_out,
                                int64_t rows, int H, float eps,
                                int rows_per_unit) {
@@ -142,7 +142,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 template <typename T, int VC, int CH>
-__global__ void rms_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+__global__ __launch_bounds__(kThreads) void rms_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dy,
                                const T* __restrict__ w,
                                const float* __restrict__ rstd_in,
                                T* __restrict__ dx, float* __restrict__ dwpart,
