@@ -451,6 +451,14 @@ int64_t sum_blocks(int64_t n) { return (n + kSumRows - 1) / kSumRows; }
 
 }  // namespace
 
+// A launch takes fewer than 2^32 threads; the second one of ce_sum_kernel
+// has one block.
+int64_t ce_max_rows(int64_t vocab) {
+  return std::min<int64_t>((int64_t{1} << 32) / plan_of(1 << 20, vocab).group -
+                               kThreads,
+                           kSumRows * kSumRows);
+}
+
 // Partial sums, the rows' losses, and statistics of segments.
 int64_t ce_scratch_bytes(int64_t n, int64_t vocab) {
   const int segs = plan_of(n, vocab).segs;

@@ -109,8 +109,8 @@ void launch_swiglu_bwd(int dtype, const void* dz, const void* a, const void* g,
 // Embedding (embedding.hip): ids int32 or int64 [n], w [vocab, dim] with rows
 // wstride values apart, y/dy [n, dim] and dw [vocab, dim] contiguous.
 // Backward scratch: keys uint64[2n], part fp32[embed_part_floats(...)];
-// padding: the id without a gradient, or -1. Needs dim > 0 and n < 2^31;
-// forward needs n > 0.
+// padding: the id without a gradient, or -1. dw's allocation is rounded up to
+// 16 bytes. Needs dim > 0 and n < 2^26; forward needs n > 0.
 int64_t embed_part_floats(int64_t n, int64_t dim, int elem_size);
 void launch_embed_fwd(int dtype, bool ids64, const void* ids, const void* w,
                       void* y, int64_t n, int64_t vocab, int64_t dim,
@@ -126,6 +126,7 @@ void launch_embed_bwd(int dtype, bool ids64, const void* ids, const void* dy,
 // (loss fp32[1]). kept fp32[2n] and factor fp32[1] (null in the backward pass
 // of reduction 0) go from forward to backward. gout: the loss's gradient, one
 // for each row (gstride 1) or one for all (0).
+int64_t ce_max_rows(int64_t vocab);
 int64_t ce_scratch_bytes(int64_t n, int64_t vocab);
 void launch_ce_fwd(int dtype, const void* x, int64_t inner,
                    int64_t stride_outer, int64_t stride_inner,

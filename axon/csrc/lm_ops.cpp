@@ -134,10 +134,11 @@ at::Tensor embedding(const at::Tensor& ids_in, const at::Tensor& weight_in,
                     weight_in.device());
   TORCH_CHECK_TYPE(float_type(weight_in),
                    "embedding: weight must be float, half or bfloat16");
+  // A launch takes fewer than 2^32 threads, 64 for each token.
   TORCH_CHECK_VALUE(vocab < (int64_t{1} << 31) && dim < (int64_t{1} << 22) &&
-                        ids_in.numel() < (int64_t{1} << 31),
-                    "embedding: fewer than 2^31 rows and ids, and rows of "
-                    "fewer than 2^22 values");
+                        ids_in.numel() < (int64_t{1} << 26),
+                    "embedding: fewer than 2^31 rows, of fewer than 2^22 "
+                    "values, and fewer than 2^26 ids");
   check_no_tangent(weight_in, "embedding");
   const Guard guard(weight_in.device());
   const at::Tensor weight = dim > 1 && weight_in.stride(1) != 1
@@ -260,11 +261,12 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
                     ", logits on ", logits.device());
   TORCH_CHECK_TYPE(float_type(logits),
                    "cross_entropy: logits must be float, half or bfloat16");
-  // The partial sums of more rows would take a third launch; places within a
-  // row are counted in 32 bits.
-  TORCH_CHECK_VALUE(target.numel() < (int64_t{1} << 28) &&
-                        logits.size(-1) < (int64_t{1} << 30),
-                    "cross_entropy: fewer than 2^28 rows and 2^30 classes");
+  // Places within a row are counted in 32 bits.
+  TORCH_CHECK_VALUE(logits.size(-1) < (int64_t{1} << 30),
+                    "cross_entropy: fewer than 2^30 classes");
+  TORCH_CHECK_VALUE(target.numel() <= ce_max_rows(logits.size(-1)),
+                    "cross_entropy: at most ", ce_max_rows(logits.size(-1)),
+                    " rows of ", logits.size(-1), " classes");
   check_no_tangent(logits, "cross_entropy");
   const Guard guard(logits.device());
   // With the caller's autograd: the gradient goes back through these.
@@ -407,8 +409,16 @@ std::vector<Table> tables_of(const std::vector<at::Tensor>& ts) {
   return tables;
 }
 
+// Strided tensors get their scaled copies; autograd learns that the others
+// were written to.
 void write_back(const Grads& g) {
-  for (auto& s : g.strided) s.first.copy_(g.dense[s.second]);
+  size_t next = 0;
+  for (size_t i = 0; i < g.dense.size(); ++i) {
+    if (next < g.strided.size() && g.strided[next].second == i)
+      g.strided[next++].first.copy_(g.dense[i]);
+    else if (!g.dense[i].is_inference())
+      g.dense[i].unsafeGetTensorImpl()->bump_version();
+  }
 }
 
 // (norm, factor) as fp32[2], and the tensors scaled by the factor if `clip`;

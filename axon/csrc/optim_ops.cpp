@@ -35,6 +35,10 @@ ChunkPlan build_chunks(const std::vector<at::Tensor>& ps,
                        const std::vector<at::Tensor>& ms,
                        const std::vector<at::Tensor>& vs,
                        float* u_base /* fp32 scratch or null */) {
+  TORCH_CHECK(ps[0].scalar_type() == at::kFloat ||
+                  ps[0].scalar_type() == at::kHalf ||
+                  ps[0].scalar_type() == at::kBFloat16,
+              "fused optimizer: float/half/bfloat16 parameters only");
   int64_t total = 0;
   for (auto& p : ps) total += p.numel();
   int64_t ce = pick_chunk_elems(total);

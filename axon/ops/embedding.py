@@ -12,7 +12,8 @@ _SUPPORTED = (torch.float32, torch.float16, torch.bfloat16)
 def embedding(ids, weight, scale=1.0, padding_idx=None):
     """scale * weight[ids], of ids' shape with weight's rows behind it.
 
-    ids: int32 or int64 of any shape; weight: [V, D]. The row `padding_idx`
+    ids: int32 or int64 of any shape; weight: [V, D]; scale: a number (a
+    tensor is refused: it would get no gradient). The row `padding_idx`
     is looked up like any other and gets no gradient. Sums in the gradient are
     in fp32, rounded once to weight's type.
 
@@ -20,6 +21,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     check would wait for the GPU); on the CPU it raises IndexError. The
     gradient is not differentiable again.
     """
+    if isinstance(scale, torch.Tensor):
+        raise TypeError("embedding: scale must be a number")
     if weight.is_cuda and weight.dtype in _SUPPORTED:
         from axon import _core
 
@@ -42,10 +45,8 @@ class FusedEmbedding(nn.Embedding):
     """nn.Embedding with the CDNA4 kernels, and a factor for its rows. Same
     state dict. max_norm, scale_grad_by_freq and sparse take torch's path."""
 
-    def __init__(self, num_embeddings, embedding_dim, padding_idx=None,
-                 scale=1.0, **kwargs):
-        super().__init__(num_embeddings, embedding_dim,
-                         padding_idx=padding_idx, **kwargs)
+    def __init__(self, *args, scale=1.0, **kwargs):
+        super().__init__(*args, **kwargs)
         self.scale = float(scale)
 
     def forward(self, input):

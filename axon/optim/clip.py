@@ -84,7 +84,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0,
     norm before clipping, a 0-dim fp32 tensor on the gradients' device.
 
     norm_type: 1, 2 or inf. A gradient that several parameters share counts
-    once and is scaled once; gradients that share memory in part are refused.
+    once and is scaled once; on the GPU, gradients that share memory in part
+    are refused.
     A norm of inf or NaN makes the factor 0 or NaN as in torch;
     error_if_nonfinite raises instead (and waits for the GPU).
 
@@ -95,7 +96,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0,
         with opt.skip_synchronize():
             opt.step()
 
-    or give the fused optimizer max_grad_norm, and step() does both.
+    or give the fused optimizer max_grad_norm, and step() does both. Under a
+    GradScaler, unscale the gradients first (scaler.unscale_(opt)), either way.
     """
     norm_type, max_norm = _checked_type(norm_type), _checked_max(max_norm)
     parameters = ([parameters] if isinstance(parameters, torch.Tensor)

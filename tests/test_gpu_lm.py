@@ -532,6 +532,19 @@ def test_clip_extremes():
     assert float(grad_norm([torch.zeros(0, device=DEV)])) == 0.0
 
 
+def test_clip_tells_autograd():
+    """What was saved before the gradients were scaled is known as stale."""
+    from axon.optim import clip_grad_norm_
+
+    p = torch.nn.Parameter(torch.zeros(8, device=DEV))
+    p.grad = torch.ones(8, device=DEV)
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    out = (w * p.grad).sum()
+    clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.backward()
+
+
 def test_clip_refusals_gpu():
     from axon.optim import clip_grad_norm_
 
@@ -738,6 +751,35 @@ def test_refusals_gpu():
         embedding(torch.zeros(3, dtype=torch.long), w)
     with pytest.raises(ValueError):
         cross_entropy(w, torch.zeros(4, dtype=torch.long))
+    many = torch.zeros(1, dtype=torch.long, device=DEV)
+    with pytest.raises(ValueError):
+        embedding(many.expand(1 << 26), w)
+    with pytest.raises(ValueError):
+        cross_entropy(w[:1, :1].expand(1 << 24, 1025), many.expand(1 << 24))
+    with pytest.raises(ValueError):
+        cross_entropy(w[0, 0].expand(1, 1 << 30), many)
+    for bad in (dict(padding_idx=4), dict(padding_idx=-5)):
+        with pytest.raises(ValueError):
+            embedding(many, w, **bad)
+    with pytest.raises(TypeError):
+        embedding(many.float(), w)
+    with pytest.raises(TypeError):
+        embedding(many, w, scale=torch.ones((), device=DEV))
+    with pytest.raises(ValueError):
+        embedding(many, w[0])
+    for bad in (dict(reduction="max"), dict(label_smoothing=1.5)):
+        with pytest.raises(ValueError):
+            cross_entropy(w, many.expand(4), **bad)
+    with pytest.raises(ValueError):
+        cross_entropy(w, many)
+    with pytest.raises(TypeError):
+        cross_entropy(w, many.expand(4).float())
+    double = torch.nn.Parameter(torch.ones(3, device=DEV,
+                                           dtype=torch.float64))
+    double.grad = torch.ones_like(double)
+    from axon.optim import FusedAdamW
+    with pytest.raises(RuntimeError):
+        FusedAdamW([double]).step()
     x = torch.randn(4, 8, device=DEV, requires_grad=True)
     loss = cross_entropy(x, torch.zeros(4, dtype=torch.long, device=DEV))
     (g,) = torch.autograd.grad(loss, x, create_graph=True)

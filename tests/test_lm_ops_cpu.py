@@ -30,6 +30,10 @@ def test_embedding_matches_torch():
     ref = torch.nn.Embedding(9, 5, padding_idx=1)
     ref.load_state_dict(m.state_dict())
     assert torch.equal(m(ids), ref(ids) * 3.0)
+    table = torch.randn(4, 3)
+    assert torch.equal(FusedEmbedding.from_pretrained(table)(ids % 4),
+                       table[ids % 4])
+    assert FusedEmbedding(9, 5, None, 2.0).max_norm == 2.0  # as nn.Embedding
     sparse = FusedEmbedding(9, 5, sparse=True)
     sparse(ids).sum().backward()
     assert sparse.weight.grad.is_sparse
@@ -42,6 +46,8 @@ def test_embedding_refusals():
         embedding(ids, w[0])
     with pytest.raises(TypeError):
         embedding(ids.float(), w)
+    with pytest.raises(TypeError):
+        embedding(ids, w, scale=torch.tensor(2.0))
     for bad in (4, -5):
         with pytest.raises(ValueError):
             embedding(ids, w, padding_idx=bad)
