@@ -23,7 +23,10 @@ constexpr int kThreads = 256;
 // ------------------------------------------------------------------ forward
 //
 // A group of `lanes` lanes copies up to kFwdVecs 16-byte vectors of one row;
-// wide rows are spread over gridDim.y. An id outside [0, V) gives a row of
+// wide rows are spread over gridDim.y. 32768 rows of 4096 bf16 from a table
+// of 128256: 72 us, 5.2 TB/s (92 us right behind a gradient, whose last zeros
+// still go to memory then); 8 rows of 2048: 2.3 us, the latency of two
+// dependent loads and a store. An id outside [0, V) gives a row of
 // NaN: the kernel reads nothing for it, and the caller sees it in the loss.
 
 constexpr int kFwdVecs = 4;
@@ -91,7 +94,9 @@ constexpr int kRankKeys = 64;  // keys that a block places, one for each lane
 constexpr int kMergeRuns = 16;
 
 // dW is filled with zeros by further blocks of the sorting launches, which
-// leave memory idle; each writes kFillUnits units of 16 bytes.
+// leave memory idle; each writes kFillUnits units of 16 bytes. (1.05 GB of
+// zeros and the keys of 32768 tokens: 80 + 98 us, 5.9 TB/s; the keys alone take
+// 11 + 12.)
 constexpr int kFillUnits = 4096;
 
 struct Fill {
@@ -242,7 +247,9 @@ __global__ __launch_bounds__(kThreads) void embed_merge_kernel(
 //
 // A chunk has 64 tokens at most: each lane loads one key, and reading them
 // from the lanes makes ids and row addresses uniform, so that changes of the
-// id are scalar branches and kRowsAhead rows are in flight.
+// id are scalar branches and kRowsAhead rows are in flight. The rows of dy are
+// read once, past the caches, which are full of dW's zeros: 32768 rows of 4096
+// bf16 take 79 us (5.0 TB/s, with the rows of dW) and took 119 through them.
 
 constexpr int kRowsAhead = 8;
 constexpr int kMaxChunk = 64;
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(
       __ballot(next == id && end + static_cast<int64_t>(lane) * chunk < n);
   int64_t last = ci + __builtin_ctzll(~on | (1ull << 63));
   if (on == ~0ull) {
-    const uint64_t after = static_cast<uint64_t>(id) + 1 << 32;
+    const uint64_t after = (static_cast<uint64_t>(id) + 1) << 32;
     last = (end + count_below(keys + end, n - end, after) - 1) / chunk;
   }
   __shared__ float s[kJoinWaves][kJoinCols][64];
