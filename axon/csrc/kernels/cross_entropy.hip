@@ -27,8 +27,8 @@ constexpr int kThreads = 256;
 constexpr float kLowest = -3.402823466e+38f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// exp by the hardware's exp2 (1 ulp), on a difference that is exact for the
-// values that matter in a sum.
+// exp by the hardware's exp2 (1 ulp; 0 below 2^-126), on a difference that is
+// exact for the values that matter in a sum.
 __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(d * kLog2e);
 }

@@ -21,13 +21,16 @@ def main():
     ap.add_argument("--batch", type=int, default=64)
     ap.add_argument("--seq", type=int, default=128)
     ap.add_argument("--steps", type=int, default=50)
+    ap.add_argument("--max-grad-norm", type=float, default=None,
+                    help="clip by the norm of the averaged gradients")
     args = ap.parse_args()
 
     hvd.init()
     device = "cuda" if torch.cuda.is_available() else "cpu"
     dtype = torch.bfloat16 if device == "cuda" else torch.float32
     model = BertForPreTraining(bert_large_config()).to(device, dtype)
-    opt = FusedLAMB(model.parameters(), lr=1e-3, weight_decay=0.01)
+    opt = FusedLAMB(model.parameters(), lr=1e-3, weight_decay=0.01,
+                    max_grad_norm=args.max_grad_norm)
     opt = hvd.DistributedOptimizer(opt, named_parameters=model.named_parameters(),
                                    compression=hvd.Compression.fp16)
     hvd.broadcast_parameters(model.state_dict(), root_rank=0)

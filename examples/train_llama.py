@@ -24,6 +24,8 @@ def main():
     ap.add_argument("--seq", type=int, default=4096)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--small", action="store_true", help="1B variant")
+    ap.add_argument("--max-grad-norm", type=float, default=None,
+                    help="clip by the norm of the averaged gradients")
     args = ap.parse_args()
 
     hvd.init()
@@ -33,7 +35,8 @@ def main():
     with torch.device(device):  # on-device init (8B fp32 on host is slow)
         model = LlamaForCausalLM(cfg)
     model = model.to(dtype=dtype)
-    opt = FusedAdamW(model.parameters(), lr=3e-4)
+    opt = FusedAdamW(model.parameters(), lr=3e-4,
+                     max_grad_norm=args.max_grad_norm)
     opt = hvd.DistributedOptimizer(opt, named_parameters=model.named_parameters())
     hvd.broadcast_parameters(model.state_dict(), root_rank=0)
 

@@ -237,6 +237,8 @@ def _loss_wanted(x, target, dloss, eps, ignore, reduction):
         tol = tol + 2 * U * fine(loss).abs()
     p_tol = p * (s_rel + U * (6 + 3 * fine(d).abs())) + 4 * U * onehot + \
         4 * U * eps / vocab + 4 * U * p
+    # The GPU's exp2 gives 0 below the least normal value, 2^-126; S >= 1.
+    p_tol = p_tol + 2.0 ** -126
     exact = _rounded(grad, x.dtype, 3)
     gtol = torch.where(torch.isfinite(p_tol), p_tol, 0.0) * \
         per_row.abs()[:, None] * (1 + torch.finfo(x.dtype).eps) + exact
