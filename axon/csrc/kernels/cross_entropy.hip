@@ -373,26 +373,36 @@ __global__ __launch_bounds__(kThreads) void ce_grad_kernel(
   for (int j = tail + t; j < len; j += G) one(j);
 }
 
-// 16 lanes for a row of up to 128 logits, a wave for one of up to 1024, a
-// block for a longer one. Where rows are too few for two blocks on each CU,
-// long ones are cut into segments of 4096 logits or more, and joined by a
-// launch of its own: 511 rows of 32003 fp16 took 8.4 us whole, 11.3 and 12.7
-// in 2 and 4 segments; 64 rows of 128256 8.1 us in 8 segments, 11.3 in 31.
+// 16 lanes for a row of up to 160 vectors of 16 bytes, a wave for one of up to
+// 1024 where there are rows enough for it, a block for a longer one. 65536
+// rows of bf16, loss and gradient: of 1100 logits 27 + 51 us by 16 lanes, 40 +
+// 63 by waves, 100 + 118 by blocks; of 8000 162 + 369 by waves, 208 + 394 by
+// blocks; of 12000 (half as many) 120 + 279 and 125 + 263.
+//
+// Where rows are too few for two blocks on each CU, long ones are cut into
+// segments of 4096 logits or more, and joined by a launch of its own: 511 rows
+// of 32003 fp16 took 8.4 us whole, 11.3 and 12.7 in 2 and 4 segments; 64 rows
+// of 128256 8.1 us in 8 segments, 11.3 in 31.
 struct Plan {
   int group;
   int segs;
   int64_t seg_len;
 };
 
-Plan plan_of(int64_t n, int64_t vocab) {
-  if (vocab <= 128) return {16, 1, vocab};
-  if (vocab <= 1024) return {64, 1, vocab};
+constexpr int kFew = 160, kSome = 1024;  // vectors of a row
+
+Plan plan_of(int64_t n, int64_t vocab, int64_t size) {
+  const int64_t vectors = vocab * size / 16;
+  if (vectors <= kFew) return {16, 1, vocab};
+  if (vectors <= kSome && (n >= 2048 || vectors <= 128)) return {64, 1, vocab};
   const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(n, 1));
   const int64_t most = std::max<int64_t>(1, vocab / 4096);
   const int64_t segs = std::min(want, most);
   const int64_t len = ((vocab + segs - 1) / segs + 15) / 16 * 16;
   return {kThreads, static_cast<int>((vocab + len - 1) / len), len};
 }
+
+int64_t size_of(int dtype) { return dtype == kFloat ? 4 : 2; }
 
 unsigned blocks_of(const Plan& p, int64_t n) {
   const int per = kThreads / p.group;
@@ -460,15 +470,15 @@ int64_t sum_blocks(int64_t n) { return (n + kSumRows - 1) / kSumRows; }
 
 // A launch takes fewer than 2^32 threads; the second one of ce_sum_kernel
 // has one block.
-int64_t ce_max_rows(int64_t vocab) {
-  return std::min<int64_t>((int64_t{1} << 32) / plan_of(1 << 20, vocab).group -
-                               kThreads,
+int64_t ce_max_rows(int dtype, int64_t vocab) {
+  const int group = plan_of(1 << 20, vocab, size_of(dtype)).group;
+  return std::min<int64_t>((int64_t{1} << 32) / group - kThreads,
                            kSumRows * kSumRows);
 }
 
 // Partial sums, the rows' losses, and statistics of segments.
-int64_t ce_scratch_bytes(int64_t n, int64_t vocab) {
-  const int segs = plan_of(n, vocab).segs;
+int64_t ce_scratch_bytes(int dtype, int64_t n, int64_t vocab) {
+  const int segs = plan_of(n, vocab, size_of(dtype)).segs;
   return sum_blocks(n) * 2 * static_cast<int64_t>(sizeof(double)) +
          n * static_cast<int64_t>(sizeof(float)) +
          (segs > 1 ? n * segs * static_cast<int64_t>(sizeof(Stat)) : 0);
@@ -480,7 +490,7 @@ void launch_ce_fwd(int dtype, const void* x, int64_t inner,
                    int64_t vocab, float eps, int reduction, void* scratch,
                    float* kept_, float* loss, float* factor,
                    hipStream_t stream) {
-  const Plan p = plan_of(n, vocab);
+  const Plan p = plan_of(n, vocab, size_of(dtype));
   const Rows rows = {inner, stride_outer, stride_inner};
   const int64_t blocks = sum_blocks(n);
   double* sums = static_cast<double*>(scratch);
@@ -519,7 +529,7 @@ void launch_ce_bwd(int dtype, const void* x, int64_t inner,
                    int64_t vocab, float eps, const float* kept,
                    const float* gout, int gstride, const float* factor,
                    void* dx, hipStream_t stream) {
-  const Plan p = plan_of(n, vocab);
+  const Plan p = plan_of(n, vocab, size_of(dtype));
   const Rows rows = {inner, stride_outer, stride_inner};
   auto* pass = dtype == kFloat  ? grad_pass<float>
                : dtype == kHalf ? grad_pass<_Float16>

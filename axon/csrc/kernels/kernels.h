@@ -126,8 +126,8 @@ void launch_embed_bwd(int dtype, bool ids64, const void* ids, const void* dy,
 // (loss fp32[1]). kept fp32[2n] and factor fp32[1] (null in the backward pass
 // of reduction 0) go from forward to backward. gout: the loss's gradient, one
 // for each row (gstride 1) or one for all (0).
-int64_t ce_max_rows(int64_t vocab);
-int64_t ce_scratch_bytes(int64_t n, int64_t vocab);
+int64_t ce_max_rows(int dtype, int64_t vocab);
+int64_t ce_scratch_bytes(int dtype, int64_t n, int64_t vocab);
 void launch_ce_fwd(int dtype, const void* x, int64_t inner,
                    int64_t stride_outer, int64_t stride_inner,
                    const int64_t* target, int64_t ignore, int64_t n,

@@ -264,8 +264,8 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
   // Places within a row are counted in 32 bits.
   TORCH_CHECK_VALUE(logits.size(-1) < (int64_t{1} << 30),
                     "cross_entropy: fewer than 2^30 classes");
-  TORCH_CHECK_VALUE(target.numel() <= ce_max_rows(logits.size(-1)),
-                    "cross_entropy: at most ", ce_max_rows(logits.size(-1)),
+  const int64_t most = ce_max_rows(code_of(logits), logits.size(-1));
+  TORCH_CHECK_VALUE(target.numel() <= most, "cross_entropy: at most ", most,
                     " rows of ", logits.size(-1), " classes");
   check_no_tangent(logits, "cross_entropy");
   const Guard guard(logits.device());
@@ -299,7 +299,7 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
                           : at::empty({}, fopt);
     // Scratch (whole doubles), and what the backward pass takes: a row's
     // (m, 1/S), and the factor at its end.
-    const int64_t scratch = (ce_scratch_bytes(r.n, r.vocab) + 7) / 8 * 2;
+    const int64_t scratch = (ce_scratch_bytes(code_of(x), r.n, r.vocab) + 7) / 8 * 2;
     at::Tensor work = at::empty({scratch + 2 * r.n + 1}, fopt);
     float* const kept = work.data_ptr<float>() + scratch;
     launch_ce_fwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,

@@ -219,7 +219,8 @@ def _loss_wanted(x, target, dloss, eps, ignore, reduction):
     # product; the result: 1 ulp = 2 u), the additions of one thread and of
     # the joins, a rescaling at each step whose arguments add up to the range.
     fine = lambda v: torch.where(torch.isfinite(v), v, 0.0)  # noqa: E731
-    steps = vocab / 64 + 16
+    # A thread has V / 16 values of a short row (up to 1280), V / 64 of others.
+    steps = min(vocab / 16, 80) + vocab / 64 + 16
     reach = fine(d).abs().amax(1, keepdim=True)
     lost = fine(p * fine(d).abs()).sum(1, keepdim=True)
     s_rel = U * (2 + 3 * lost + 3 * steps + 3 * reach)
@@ -275,6 +276,7 @@ def _logits(n, vocab, dtype, seed=0, std=3.0):
 @pytest.mark.parametrize("n,vocab", [
     (1, 1), (1, 2), (5, 7), (64, 10), (33, 255), (9, 1000), (4, 1024),
     (4, 1025), (3, 4099), (130, 2051), (1, 50001), (2, 131072), (700, 8191),
+    (2100, 1281), (2100, 2600), (2500, 8200), (513, 641), (20, 1280),
 ])
 def test_cross_entropy(n, vocab, dtype):
     x, t, g = _logits(n, vocab, dtype)
@@ -757,7 +759,7 @@ def test_refusals_gpu():
     with pytest.raises(ValueError):
         embedding(many.expand(1 << 26), w)
     with pytest.raises(ValueError):
-        cross_entropy(w[:1, :1].expand(1 << 24, 1025), many.expand(1 << 24))
+        cross_entropy(w[:1, :1].expand(1 << 24, 5000), many.expand(1 << 24))
     with pytest.raises(ValueError):
         cross_entropy(w[0, 0].expand(1, 1 << 30), many)
     for bad in (dict(padding_idx=4), dict(padding_idx=-5)):
