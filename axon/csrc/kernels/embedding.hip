@@ -209,31 +209,36 @@ __device__ __forceinline__ int64_t count_below(const uint64_t* p, int64_t n,
   return lo;
 }
 
-__global__ __launch_bounds__(kThreads) void embed_merge_kernel(
+// A block places 64 keys, which stand next to each other in one run: wave r
+// bisects run r for all of them, along nearly the same path.
+__global__ __launch_bounds__(kMergeRuns * 64) void embed_merge_kernel(
     const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int64_t n,
     int64_t run, int64_t blocks, Fill f) {
   bool fills;
   const int64_t block = kind_of(blockIdx.x, blocks, f.blocks(), &fills);
   if (fills) {
-    fill<kThreads>(f, block);
+    fill<kMergeRuns * 64>(f, block);
     return;
   }
-  const int64_t i = (block * kThreads + threadIdx.x) / kMergeRuns;
-  const int r = threadIdx.x % kMergeRuns;
-  const bool on = i < n;
-  const uint64_t key = on ? in[i] : 0;
-  const int64_t group = i / (run * kMergeRuns) * (run * kMergeRuns);
-  const int64_t mine = i / run * run;
+  __shared__ int64_t places[kMergeRuns][64];
+  const int r = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t i = block * 64 + lane;
+  const int64_t at = min(i, n - 1);
+  const uint64_t key = in[at];
+  const int64_t group = at / (run * kMergeRuns) * (run * kMergeRuns);
+  const int64_t mine = at / run * run;
   const int64_t start = group + r * run;
-  int64_t place = 0;
-  if (on && start == mine)
-    place = group + (i - mine);
-  else if (on && start < n)
-    place = count_below(in + start, min(run, n - start), key);
+  places[r][lane] =
+      start == mine ? group + (at - mine)
+      : start < n   ? count_below(in + start, min(run, n - start), key)
+                    : 0;
+  __syncthreads();
+  if (r == 0 && i < n) {
+    int64_t place = 0;
 #pragma unroll
-  for (int off = kMergeRuns / 2; off > 0; off >>= 1)
-    place += __shfl_xor(place, off, 64);
-  if (on && r == 0) out[place] = key;
+    for (int w = 0; w < kMergeRuns; ++w) place += places[w][lane];
+    out[place] = key;
+  }
 }
 
 // ------------------------------------------------------------ summing rows
@@ -254,8 +259,13 @@ __global__ __launch_bounds__(kThreads) void embed_merge_kernel(
 constexpr int kRowsAhead = 8;
 constexpr int kMaxChunk = 64;
 
-// kTail: rows that are no whole number of 16-byte vectors.
-template <typename T, bool kTail>
+// kRows: rows are whole 16-byte vectors (kWhole); or their last vector is not
+// (kTail), and its lane reads a whole one that ends with the row, of whose
+// columns the first kept ones are the lane's before; or they are shorter than
+// a vector (kNarrow).
+enum { kWhole, kTail, kNarrow };
+
+template <typename T, int kRows>
 __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
     const uint64_t* __restrict__ keys, const T* __restrict__ dy,
     T* __restrict__ dw, float* __restrict__ part, int64_t n, int64_t vocab,
@@ -266,11 +276,13 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t ci = unit / slices;
   if (ci >= nchunks) return;
-  const int64_t c0 = (unit % slices) * 64 * V + lane * V;
+  const int64_t column = (unit % slices) * 64 * V + lane * V;
+  const bool active = column < dim;
+  const int64_t c0 = kRows == kTail ? min(column, dim - V) : column;
+  const int kept = kRows == kTail ? static_cast<int>(column - c0) : 0;
+  const int width = kRows == kNarrow ? static_cast<int>(dim) : V;
   const int64_t begin = ci * chunk;
   const int len = static_cast<int>(min<int64_t>(chunk, n - begin));
-  const int width =
-      c0 >= dim ? 0 : static_cast<int>(min<int64_t>(V, dim - c0));
 
   const uint64_t mine = lane < len ? keys[begin + lane] : ~0ull;
   const uint32_t none = static_cast<uint32_t>(vocab);
@@ -295,27 +307,27 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
   bool first = before == cur;
 
   auto flush = [&](bool goes_on) {
-    if (cur == none) return;
+    if (cur == none || !active) return;
     if (first || goes_on) {
       float* p = part + (ci * 2 + (first ? 0 : 1)) * dim + c0;
-      if (width == V) {
+      if (kRows == kWhole || (kRows == kTail && kept == 0)) {
 #pragma unroll
         for (int i = 0; i < V; i += 4) store16(p + i, pack<float>(acc + i));
-      } else if (kTail) {
+      } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          if (i < width) p[i] = acc[i];
+          if (i >= kept && i < width) p[i] = acc[i];
       }
     } else {
       T* p = dw + static_cast<int64_t>(cur) * dim + c0;
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] *= scale;
-      if (width == V) {
+      if (kRows == kWhole || (kRows == kTail && kept == 0)) {
         store16(p, pack<T>(acc));
-      } else if (kTail) {
+      } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          if (i < width) p[i] = static_cast<T>(acc[i]);
+          if (i >= kept && i < width) p[i] = static_cast<T>(acc[i]);
       }
     }
   };
@@ -327,9 +339,9 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
       r[k] = u32x4{0, 0, 0, 0};
       if (p0 + k < len && id_at(p0 + k) != none) {
         const T* src = dy + static_cast<int64_t>(row_at(p0 + k)) * dim + c0;
-        if (width == V) {
-          r[k] = load16_once(src);
-        } else if (kTail && width > 0) {
+        if (kRows != kNarrow) {
+          if (active) r[k] = load16_once(src);
+        } else if (active) {
           T t[V] = {};
 #pragma unroll
           for (int i = 0; i < V; ++i)
@@ -476,17 +488,18 @@ void bwd(const I* ids, const T* dy, T* dw, uint64_t* keys, float* part,
   uint64_t* other = keys + n;
   for (int64_t run = kTile; run < n; run *= kMergeRuns) {
     f = next_fill();
-    const int64_t blocks = (n * kMergeRuns + kThreads - 1) / kThreads;
+    const int64_t blocks = (n + 63) / 64;
     hipLaunchKernelGGL(embed_merge_kernel,
                        dim3(static_cast<unsigned>(blocks + f.blocks())),
-                       dim3(kThreads), 0, stream, keys, other, n, run, blocks,
+                       dim3(kMergeRuns * 64), 0, stream, keys, other, n, run, blocks,
                        f);
     std::swap(keys, other);
   }
   const SumPlan p = sum_plan(n, dim, kVec<T>);
   const int64_t units = p.nchunks * p.slices;
-  auto* sum = dim % kVec<T> ? &embed_sum_kernel<T, true>
-                            : &embed_sum_kernel<T, false>;
+  auto* sum = dim % kVec<T> == 0 ? &embed_sum_kernel<T, kWhole>
+              : dim > kVec<T>   ? &embed_sum_kernel<T, kTail>
+                                : &embed_sum_kernel<T, kNarrow>;
   hipLaunchKernelGGL(sum, dim3(static_cast<unsigned>((units + 3) / 4)),
                      dim3(kThreads), 0, stream, keys, dy, dw, part, n, vocab,
                      dim, p.chunk, p.nchunks, p.slices, scale);
