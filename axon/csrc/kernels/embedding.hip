@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
 // equal ones before it. All pairs are compared, a tile's length for each
 // token, but over the whole chip and without a barrier in between: a bitonic
 // sort of 2048 keys by one block took 15 us, the count takes 5. (A tile of
-// 8192 would save their merge, but took 22 us instead of 9 and 10.) Then runs
+// 8192 would save their merge, but took 22 us instead of 9 and 7.) Then runs
 // are merged, up to kMergeRuns at a time: a key's place in
 // the merged run is its place in its own run plus the number of smaller keys
 // in each of the others, one lane for each run and a bisection of dependent
@@ -95,8 +95,8 @@ constexpr int kMergeRuns = 16;
 
 // dW is filled with zeros by further blocks of the sorting launches, which
 // leave memory idle; each writes kFillUnits units of 16 bytes. (1.05 GB of
-// zeros and the keys of 32768 tokens: 80 + 98 us, 5.9 TB/s; the keys alone take
-// 11 + 12.)
+// zeros and the keys of 32768 tokens: 82 + 94 us, 6.0 TB/s; the keys alone take
+// 11 + 7.)
 constexpr int kFillUnits = 4096;
 
 struct Fill {
