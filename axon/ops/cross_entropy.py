@@ -20,7 +20,9 @@ def cross_entropy(logits, target, ignore_index=-100, label_smoothing=0.0,
 
     On the GPU a label outside [0, V) that is not ignore_index makes the loss
     and its row's gradient NaN (a check would wait for the GPU); on the CPU it
-    raises IndexError. The gradient is not differentiable again.
+    raises IndexError. A call on the GPU takes up to 2^24 - 256 rows, 2^26 -
+    256 of up to 1024 vectors of 16 bytes. The gradient is not differentiable
+    again.
     """
     if logits.is_cuda and logits.dtype in _SUPPORTED:
         from axon import _core

@@ -18,8 +18,9 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     in fp32, rounded once to weight's type.
 
     On the GPU an id outside [0, V) gives a row of NaN and no gradient (a
-    check would wait for the GPU); on the CPU it raises IndexError. The
-    gradient is not differentiable again.
+    check would wait for the GPU); on the CPU it raises IndexError. A call on
+    the GPU takes fewer than 2^26 ids. The gradient is not differentiable
+    again.
     """
     if isinstance(scale, torch.Tensor):
         raise TypeError("embedding: scale must be a number")

@@ -113,6 +113,15 @@ def test_embedding_no_tokens():
     from axon.ops import embedding
 
     w = torch.randn(5, 8, device=DEV, requires_grad=True)
+    one = embedding(torch.tensor(3, device=DEV), w)  # a single id
+    assert torch.equal(one, w[3])
+    empty = torch.zeros(0, 8, device=DEV, requires_grad=True)
+    rows = embedding(torch.tensor([0, 1], device=DEV), empty)  # no table
+    assert rows.isnan().all()
+    rows.sum().backward()
+    assert empty.grad.shape == (0, 8)
+
+    w = torch.randn(5, 8, device=DEV, requires_grad=True)
     out = embedding(torch.zeros(2, 0, dtype=torch.long, device=DEV), w)
     assert out.shape == (2, 0, 8)
     out.sum().backward()
@@ -351,6 +360,12 @@ def test_cross_entropy_layouts(dtype):
     x4 = base.reshape(3, 2, 4, 70)
     assert torch.equal(cross_entropy(x4, t.view(3, 2, 4), reduction="none"),
                        cross_entropy(base, t, reduction="none").view(3, 2, 4))
+    # The gradient of a sum has one value for all rows.
+    x = base[0].clone().requires_grad_()
+    cross_entropy(x, t[0], reduction="none").sum().backward()
+    y = base[0].clone().requires_grad_()
+    cross_entropy(y, t[0], reduction="sum").backward()
+    assert torch.equal(x.grad, y.grad)
     none = cross_entropy(base[:0].requires_grad_(), t[:0], reduction="sum")
     assert float(none.detach()) == 0.0
 
