@@ -2,9 +2,17 @@
 // (kernels/embedding.hip), cross entropy (kernels/cross_entropy.hip) and the
 // gradient norm (kernels/grad_norm.hip). They run on the tensors' device, on
 // its current torch stream; scratch comes from torch's allocator per call.
+//
+// Each one that gives new tensors is an operator of torch's dispatcher
+// (axon::...), its backward pass too. What records calls there (torch.jit.trace,
+// make_fx, a profiler) or transforms them (vmap, torch.func) then sees the
+// operator and its inputs; in a call that goes past the dispatcher it sees only
+// how the output is allocated, and a trace of that returns memory that nothing
+// wrote. The dispatcher costs a call about 0.1 us (a lookup 4.2 us).
 #include <torch/extension.h>
 
 #include <ATen/MemoryOverlap.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -14,6 +22,10 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <torch/library.h>
+
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <algorithm>
 #include <mutex>
@@ -33,9 +45,8 @@ hipStream_t stream_of(const at::Tensor& t) {
 
 int code_of(const at::Tensor& t) { return static_cast<int>(t.scalar_type()); }
 
-bool float_type(const at::Tensor& t) {
-  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
-         t.scalar_type() == at::kBFloat16;
+bool float_type(at::ScalarType t) {
+  return t == at::kFloat || t == at::kHalf || t == at::kBFloat16;
 }
 
 void check_launch() {
@@ -58,17 +69,92 @@ void check_no_tangent(const at::Tensor& t, const char* what) {
                               ": no forward-mode derivative");
 }
 
+// What reads and writes the parameters' .grad is no function of its arguments.
+void check_untraced(const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !torch::jit::tracer::isTracing() &&
+          !c10::impl::TorchDispatchModeTLS::get_mode(
+               c10::impl::TorchDispatchModeKey::PROXY)
+               .has_value(),
+      what, ": cannot be traced");
+}
+
+// An operator of the dispatcher, by its name.
+template <typename Signature>
+c10::TypedOperatorHandle<Signature> op_of(const char* name) {
+  return c10::Dispatcher::singleton()
+      .findSchemaOrThrow(name, "")
+      .typed<Signature>();
+}
+
 // The nodes below are written against torch's graph itself: a Python
 // autograd.Function costs about 20 us for each pass through it, more than
 // the kernels of a small batch.
 
 // ------------------------------------------------------------- embedding
 
-at::Tensor embed_bwd(const at::Tensor& ids, const at::Tensor& dy_in,
-                     int64_t vocab, int64_t padding, double scale) {
+void check_embedding(const at::Tensor& ids, at::ScalarType type, int64_t vocab,
+                     int64_t dim) {
+  TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong ||
+                       ids.scalar_type() == at::kInt,
+                   "embedding: ids must be int32 or int64, got ",
+                   ids.scalar_type());
+  TORCH_CHECK_TYPE(float_type(type),
+                   "embedding: weight must be float, half or bfloat16");
+  // A launch takes fewer than 2^32 threads, 64 for each token.
+  TORCH_CHECK_VALUE(vocab < (int64_t{1} << 31) && dim < (int64_t{1} << 22) &&
+                        ids.numel() < (int64_t{1} << 26),
+                    "embedding: fewer than 2^31 rows, of fewer than 2^22 "
+                    "values, and fewer than 2^26 ids");
+}
+
+at::Tensor embedding_kernel(const at::Tensor& ids_in,
+                            const at::Tensor& weight_in, double scale,
+                            c10::optional<int64_t> padding_idx) {
+  TORCH_CHECK_VALUE(weight_in.dim() == 2, "embedding: weight must be [V, D], "
+                    "got ", weight_in.sizes());
+  const int64_t vocab = weight_in.size(0), dim = weight_in.size(1);
+  TORCH_CHECK_VALUE(!padding_idx.has_value() ||
+                        (*padding_idx >= -vocab && *padding_idx < vocab),
+                    "embedding: padding_idx ", padding_idx.value_or(0),
+                    " outside the ", vocab, " rows");
+  TORCH_CHECK_VALUE(weight_in.is_cuda() && ids_in.device() == weight_in.device(),
+                    "embedding: ids on ", ids_in.device(), ", weight on ",
+                    weight_in.device());
+  check_embedding(ids_in, weight_in.scalar_type(), vocab, dim);
+  const Guard guard(weight_in.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const at::Tensor weight = dim > 1 && weight_in.stride(1) != 1
+                                ? weight_in.contiguous()
+                                : weight_in;
+  const at::Tensor ids = ids_in.contiguous();
+  auto shape = ids.sizes().vec();
+  shape.push_back(dim);
+  at::Tensor y = at::empty(shape, weight.options());
+  if (y.numel()) {
+    launch_embed_fwd(code_of(weight), ids.scalar_type() == at::kLong,
+                     ids.data_ptr(), weight.data_ptr(), y.data_ptr(),
+                     ids.numel(), vocab, dim, weight.stride(0),
+                     static_cast<float>(scale), stream_of(weight));
+    check_launch();
+  }
+  return y;
+}
+
+// padding: the row without a gradient, or -1.
+at::Tensor embedding_backward_kernel(const at::Tensor& ids_in,
+                                     const at::Tensor& dy_in, int64_t vocab,
+                                     int64_t padding, double scale) {
+  TORCH_CHECK_VALUE(dy_in.is_cuda() && ids_in.device() == dy_in.device() &&
+                        dy_in.dim() == ids_in.dim() + 1 && vocab >= 0 &&
+                        dy_in.sizes().slice(0, ids_in.dim()) == ids_in.sizes(),
+                    "embedding: ids ", ids_in.sizes(), " and gradient ",
+                    dy_in.sizes());
+  const int64_t n = ids_in.numel(), dim = dy_in.size(-1);
+  check_embedding(ids_in, dy_in.scalar_type(), vocab, dim);
   const Guard guard(dy_in.device());
-  const at::Tensor dy = dy_in.contiguous();
-  const int64_t n = ids.numel(), dim = dy.size(-1);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const at::Tensor dy = dy_in.contiguous(), ids = ids_in.contiguous();
   // Whole units of 16 bytes, as the kernels fill it.
   const int64_t unit = 16 / static_cast<int64_t>(dy.element_size());
   at::Tensor dw =
@@ -83,8 +169,9 @@ at::Tensor embed_bwd(const at::Tensor& ids, const at::Tensor& dy_in,
   float* const part = scratch.data_ptr<float>() + 4 * n;
   launch_embed_bwd(code_of(dy), ids.scalar_type() == at::kLong, ids.data_ptr(),
                    dy.data_ptr(), dw.data_ptr(),
-                   reinterpret_cast<uint64_t*>(scratch.data_ptr()), part, n, vocab, dim, padding,
-                   static_cast<float>(scale), stream_of(dy));
+                   reinterpret_cast<uint64_t*>(scratch.data_ptr()), part, n,
+                   vocab, dim, padding, static_cast<float>(scale),
+                   stream_of(dy));
   check_launch();
   return dw;
 }
@@ -96,13 +183,15 @@ struct EmbeddingBackward : public torch::autograd::Node {
 
   torch::autograd::variable_list apply(
       torch::autograd::variable_list&& grads) override {
+    static const auto op = op_of<decltype(embedding_backward_kernel)>(
+        "axon::embedding_backward");
     std::lock_guard<std::mutex> lock(mutex_);
     const at::Tensor i = ids.unpack(shared_from_this());
     if (!grads[0].defined()) return {at::Tensor()};
     at::Tensor dw;
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      dw = embed_bwd(i, grads[0], vocab, padding, scale);
+      dw = op.call(i, grads[0], vocab, padding, scale);
     }
     return {once(dw, "embedding")};
   }
@@ -113,63 +202,31 @@ struct EmbeddingBackward : public torch::autograd::Node {
   std::string name() const override { return "AxonEmbeddingBackward"; }
 };
 
-at::Tensor embedding(const at::Tensor& ids_in, const at::Tensor& weight_in,
+at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight,
                      double scale, c10::optional<int64_t> padding_idx) {
-  TORCH_CHECK_VALUE(weight_in.dim() == 2, "embedding: weight must be [V, D], "
-                    "got ", weight_in.sizes());
-  TORCH_CHECK_TYPE(ids_in.scalar_type() == at::kLong ||
-                       ids_in.scalar_type() == at::kInt,
-                   "embedding: ids must be int32 or int64, got ",
-                   ids_in.scalar_type());
-  const int64_t vocab = weight_in.size(0), dim = weight_in.size(1);
-  int64_t padding = -1;
-  if (padding_idx.has_value()) {
-    TORCH_CHECK_VALUE(*padding_idx >= -vocab && *padding_idx < vocab,
-                      "embedding: padding_idx ", *padding_idx, " outside the ",
-                      vocab, " rows");
-    padding = *padding_idx < 0 ? *padding_idx + vocab : *padding_idx;
-  }
-  TORCH_CHECK_VALUE(weight_in.is_cuda() && ids_in.device() == weight_in.device(),
-                    "embedding: ids on ", ids_in.device(), ", weight on ",
-                    weight_in.device());
-  TORCH_CHECK_TYPE(float_type(weight_in),
-                   "embedding: weight must be float, half or bfloat16");
-  // A launch takes fewer than 2^32 threads, 64 for each token.
-  TORCH_CHECK_VALUE(vocab < (int64_t{1} << 31) && dim < (int64_t{1} << 22) &&
-                        ids_in.numel() < (int64_t{1} << 26),
-                    "embedding: fewer than 2^31 rows, of fewer than 2^22 "
-                    "values, and fewer than 2^26 ids");
-  check_no_tangent(weight_in, "embedding");
-  const Guard guard(weight_in.device());
-  const at::Tensor weight = dim > 1 && weight_in.stride(1) != 1
-                                ? weight_in.contiguous()
-                                : weight_in;
-  const at::Tensor ids = ids_in.contiguous();
-  std::shared_ptr<EmbeddingBackward> node;
-  if (torch::autograd::compute_requires_grad(weight)) {
-    node = std::shared_ptr<EmbeddingBackward>(new EmbeddingBackward(),
-                                              torch::autograd::deleteNode);
-    node->set_next_edges(torch::autograd::collect_next_edges(weight));
-    node->ids = torch::autograd::SavedVariable(ids, false);
-    node->vocab = vocab;
-    node->padding = padding;
-    node->scale = scale;
-  }
+  static const auto op = op_of<decltype(embedding_kernel)>("axon::embedding");
+  return op.call(ids, weight, scale, padding_idx);
+}
+
+at::Tensor embedding_autograd(const at::Tensor& ids, const at::Tensor& weight,
+                              double scale,
+                              c10::optional<int64_t> padding_idx) {
+  check_no_tangent(weight, "embedding");
   at::Tensor y;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto shape = ids.sizes().vec();
-    shape.push_back(dim);
-    y = at::empty(shape, weight.options());
+    y = embedding(ids, weight, scale, padding_idx);
   }
-  if (y.numel()) {
-    launch_embed_fwd(code_of(weight), ids.scalar_type() == at::kLong,
-                     ids.data_ptr(), weight.data_ptr(), y.data_ptr(),
-                     ids.numel(), vocab, dim, weight.stride(0),
-                     static_cast<float>(scale), stream_of(weight));
-    check_launch();
-  }
-  if (node) torch::autograd::set_history(y, node);
+  if (!torch::autograd::compute_requires_grad(weight)) return y;
+  auto node = std::shared_ptr<EmbeddingBackward>(new EmbeddingBackward(),
+                                                 torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(weight));
+  node->ids = torch::autograd::SavedVariable(ids, false);
+  node->vocab = weight.size(0);
+  const int64_t row = padding_idx.value_or(-1);
+  node->padding = padding_idx.has_value() && row < 0 ? row + node->vocab : row;
+  node->scale = scale;
+  torch::autograd::set_history(y, node);
   return y;
 }
 
@@ -191,60 +248,10 @@ LogitRows logit_rows(const at::Tensor& x, const at::Tensor& target) {
   return r;
 }
 
-struct CrossEntropyBackward : public torch::autograd::Node {
-  torch::autograd::SavedVariable logits, target;
-  at::Tensor kept;  // of this file alone: from kept_at on
-  int64_t kept_at = 0;
-  int64_t ignore = 0;
-  double eps = 0.0;
-  int reduction = 1;
-
-  torch::autograd::variable_list apply(
-      torch::autograd::variable_list&& grads) override {
-    std::lock_guard<std::mutex> lock(mutex_);
-    const at::Tensor x = logits.unpack(), t = target.unpack();
-    if (!grads[0].defined()) return {at::Tensor()};
-    at::Tensor dx;
-    {
-      at::AutoDispatchBelowADInplaceOrView below;
-      const LogitRows r = logit_rows(x, t);
-      const Guard guard(x.device());
-      const at::Tensor g = grads[0].contiguous();
-      TORCH_CHECK(g.is_cuda() && g.scalar_type() == at::kFloat &&
-                      g.numel() == (reduction == 0 ? r.n : 1),
-                  "cross_entropy: the loss's gradient");
-      dx = at::empty(x.sizes(), x.options());
-      const float* const k = kept.data_ptr<float>() + kept_at;
-      if (r.n > 0) {
-        launch_ce_bwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
-                      r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n,
-                      r.vocab, static_cast<float>(eps),
-                      k, g.data_ptr<float>(), reduction == 0 ? 1 : 0,
-                      reduction == 0 ? nullptr : k + 2 * r.n,
-                      dx.data_ptr(), stream_of(x));
-        check_launch();
-      }
-    }
-    return {once(dx, "cross_entropy")};
-  }
-  void release_variables() override {
-    std::lock_guard<std::mutex> lock(mutex_);
-    logits.reset_data();
-    target.reset_data();
-    kept.reset();
-  }
-  std::string name() const override { return "AxonCrossEntropyBackward"; }
-};
-
-at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
-                         int64_t ignore, double eps,
-                         const std::string& reduction_name) {
-  const int reduction = reduction_name == "none"   ? 0
-                        : reduction_name == "mean" ? 1
-                        : reduction_name == "sum"  ? 2
-                                                   : -1;
-  TORCH_CHECK_VALUE(reduction >= 0, "cross_entropy: reduction '",
-                    reduction_name, "', expected 'none', 'mean' or 'sum'");
+void check_cross_entropy(const at::Tensor& logits, const at::Tensor& target,
+                         double eps, int64_t reduction) {
+  TORCH_CHECK_VALUE(reduction >= 0 && reduction <= 2,
+                    "cross_entropy: reduction ", reduction);
   TORCH_CHECK_VALUE(eps >= 0.0 && eps <= 1.0,
                     "cross_entropy: label_smoothing outside [0, 1]: ", eps);
   TORCH_CHECK_TYPE(target.scalar_type() == at::kLong ||
@@ -259,7 +266,7 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
   TORCH_CHECK_VALUE(logits.is_cuda() && target.device() == logits.device(),
                     "cross_entropy: target on ", target.device(),
                     ", logits on ", logits.device());
-  TORCH_CHECK_TYPE(float_type(logits),
+  TORCH_CHECK_TYPE(float_type(logits.scalar_type()),
                    "cross_entropy: logits must be float, half or bfloat16");
   // Places within a row are counted in 32 bits.
   TORCH_CHECK_VALUE(logits.size(-1) < (int64_t{1} << 30),
@@ -267,9 +274,11 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
   const int64_t most = ce_max_rows(code_of(logits), logits.size(-1));
   TORCH_CHECK_VALUE(target.numel() <= most, "cross_entropy: at most ", most,
                     " rows of ", logits.size(-1), " classes");
-  check_no_tangent(logits, "cross_entropy");
-  const Guard guard(logits.device());
-  // With the caller's autograd: the gradient goes back through these.
+}
+
+// The logits and labels as the kernels take them.
+std::pair<at::Tensor, at::Tensor> dense_rows(const at::Tensor& logits,
+                                             const at::Tensor& target) {
   at::Tensor x = logits, t = target;
   if (x.size(-1) > 1 && x.stride(-1) != 1) x = x.contiguous();
   if (x.dim() > 3) {
@@ -277,43 +286,151 @@ at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
     t = t.flatten(0, -2);
   }
   if (t.scalar_type() != at::kLong) t = t.to(at::kLong);
-  t = t.contiguous();
+  return {x, t.contiguous()};
+}
+
+// Scratch of the forward pass, in floats (whole doubles).
+int64_t scratch_floats(const at::Tensor& x, const LogitRows& r) {
+  return (ce_scratch_bytes(code_of(x), r.n, r.vocab) + 7) / 8 * 2;
+}
+
+// The loss, and what the backward pass takes: behind the scratch, a row's
+// (m, 1/S), and the factor at its end. reduction: 0 none, 1 mean, 2 sum.
+std::tuple<at::Tensor, at::Tensor> cross_entropy_kernel(
+    const at::Tensor& logits, const at::Tensor& target, int64_t ignore,
+    double eps, int64_t reduction) {
+  check_cross_entropy(logits, target, eps, reduction);
+  const Guard guard(logits.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto [x, t] = dense_rows(logits, target);
   const LogitRows r = logit_rows(x, t);
-  std::shared_ptr<CrossEntropyBackward> node;
-  if (torch::autograd::compute_requires_grad(x)) {
-    node = std::shared_ptr<CrossEntropyBackward>(new CrossEntropyBackward(),
-                                                 torch::autograd::deleteNode);
-    node->set_next_edges(torch::autograd::collect_next_edges(x));
-    node->logits = torch::autograd::SavedVariable(x, false);
-    node->target = torch::autograd::SavedVariable(t, false);
-    node->ignore = ignore;
-    node->eps = eps;
-    node->reduction = reduction;
+  const auto fopt = x.options().dtype(at::kFloat);
+  // The loss, which its user may change in place, is memory of its own.
+  at::Tensor loss = reduction == 0 ? at::empty(target.sizes(), fopt)
+                                   : at::empty({}, fopt);
+  const int64_t scratch = scratch_floats(x, r);
+  at::Tensor work = at::empty({scratch + 2 * r.n + 1}, fopt);
+  float* const kept = work.data_ptr<float>() + scratch;
+  launch_ce_fwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
+                r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n, r.vocab,
+                static_cast<float>(eps), static_cast<int>(reduction),
+                work.data_ptr(), kept, loss.data_ptr<float>(), kept + 2 * r.n,
+                stream_of(x));
+  check_launch();
+  return {loss, work};
+}
+
+at::Tensor cross_entropy_backward_kernel(
+    const at::Tensor& grad, const at::Tensor& logits, const at::Tensor& target,
+    const at::Tensor& kept, int64_t ignore, double eps, int64_t reduction) {
+  check_cross_entropy(logits, target, eps, reduction);
+  const Guard guard(logits.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto [x, t] = dense_rows(logits, target);
+  const LogitRows r = logit_rows(x, t);
+  const at::Tensor g = grad.contiguous();
+  const int64_t scratch = scratch_floats(x, r);
+  for (const at::Tensor* f : {&g, &kept})
+    TORCH_CHECK(f->device() == x.device() && f->scalar_type() == at::kFloat,
+                "cross_entropy: the loss's gradient");
+  TORCH_CHECK(g.numel() == (reduction == 0 ? r.n : 1) &&
+                  kept.is_contiguous() &&
+                  kept.numel() == scratch + 2 * r.n + 1,
+              "cross_entropy: the loss's gradient");
+  at::Tensor dx = at::empty(logits.sizes(), x.options());
+  if (r.n > 0) {
+    const float* const k = kept.data_ptr<float>() + scratch;
+    launch_ce_bwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
+                  r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n, r.vocab,
+                  static_cast<float>(eps), k, g.data_ptr<float>(),
+                  reduction == 0 ? 1 : 0,
+                  reduction == 0 ? nullptr : k + 2 * r.n, dx.data_ptr(),
+                  stream_of(x));
+    check_launch();
   }
-  at::Tensor loss;
+  return dx;
+}
+
+struct CrossEntropyBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable logits, target;
+  at::Tensor kept;  // of this file alone
+  int64_t ignore = 0;
+  double eps = 0.0;
+  int64_t reduction = 1;
+
+  torch::autograd::variable_list apply(
+      torch::autograd::variable_list&& grads) override {
+    static const auto op = op_of<decltype(cross_entropy_backward_kernel)>(
+        "axon::cross_entropy_backward");
+    std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor x = logits.unpack(), t = target.unpack();
+    if (!grads[0].defined()) return {at::Tensor()};
+    at::Tensor dx;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      dx = op.call(grads[0], x, t, kept, ignore, eps, reduction);
+    }
+    return {once(dx, "cross_entropy")};
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    logits.reset_data();
+    target.reset_data();
+    kept.reset();
+  }
+  std::string name() const override { return "AxonCrossEntropyBackward"; }
+};
+
+std::tuple<at::Tensor, at::Tensor> call_cross_entropy(
+    const at::Tensor& logits, const at::Tensor& target, int64_t ignore,
+    double eps, int64_t reduction) {
+  static const auto op =
+      op_of<decltype(cross_entropy_kernel)>("axon::cross_entropy");
+  return op.call(logits, target, ignore, eps, reduction);
+}
+
+std::tuple<at::Tensor, at::Tensor> cross_entropy_autograd(
+    const at::Tensor& logits, const at::Tensor& target, int64_t ignore,
+    double eps, int64_t reduction) {
+  check_no_tangent(logits, "cross_entropy");
+  if (!torch::autograd::compute_requires_grad(logits)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_cross_entropy(logits, target, ignore, eps, reduction);
+  }
+  check_cross_entropy(logits, target, eps, reduction);
+  // With the caller's autograd: the gradient goes back through these, and the
+  // backward pass has them as the kernels take them.
+  const auto [x, t] = dense_rows(logits, target);
+  at::Tensor loss, kept;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto fopt = x.options().dtype(at::kFloat);
-    // The loss, which its user may change in place, is memory of its own.
-    loss = reduction == 0 ? at::empty(target.sizes(), fopt)
-                          : at::empty({}, fopt);
-    // Scratch (whole doubles), and what the backward pass takes: a row's
-    // (m, 1/S), and the factor at its end.
-    const int64_t scratch = (ce_scratch_bytes(code_of(x), r.n, r.vocab) + 7) / 8 * 2;
-    at::Tensor work = at::empty({scratch + 2 * r.n + 1}, fopt);
-    float* const kept = work.data_ptr<float>() + scratch;
-    launch_ce_fwd(code_of(x), x.data_ptr(), r.inner, r.stride_outer,
-                  r.stride_inner, t.data_ptr<int64_t>(), ignore, r.n, r.vocab,
-                  static_cast<float>(eps), reduction, work.data_ptr(), kept,
-                  loss.data_ptr<float>(), kept + 2 * r.n, stream_of(x));
-    check_launch();
-    if (node) {
-      node->kept = work;
-      node->kept_at = scratch;
-    }
+    std::tie(loss, kept) = call_cross_entropy(x, t, ignore, eps, reduction);
   }
-  if (node) torch::autograd::set_history(loss, node);
-  return loss;
+  auto node = std::shared_ptr<CrossEntropyBackward>(
+      new CrossEntropyBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x));
+  node->logits = torch::autograd::SavedVariable(x, false);
+  node->target = torch::autograd::SavedVariable(t, false);
+  node->kept = kept;
+  node->ignore = ignore;
+  node->eps = eps;
+  node->reduction = reduction;
+  torch::autograd::set_history(loss, node);
+  if (reduction == 0 && logits.dim() > 3) loss = loss.view(target.sizes());
+  return {loss, kept};
+}
+
+at::Tensor cross_entropy(const at::Tensor& logits, const at::Tensor& target,
+                         int64_t ignore, double eps,
+                         const std::string& reduction_name) {
+  const int reduction = reduction_name == "none"   ? 0
+                        : reduction_name == "mean" ? 1
+                        : reduction_name == "sum"  ? 2
+                                                   : -1;
+  TORCH_CHECK_VALUE(reduction >= 0, "cross_entropy: reduction '",
+                    reduction_name, "', expected 'none', 'mean' or 'sum'");
+  return std::get<0>(
+      call_cross_entropy(logits, target, ignore, eps, reduction));
 }
 
 // ---------------------------------------------------------- gradient norm
@@ -326,12 +443,12 @@ struct Grads {
   std::vector<std::pair<at::Tensor, size_t>> strided;  // original, its copy
 };
 
-Grads collect(const std::vector<at::Tensor>& ts, bool written) {
+Grads collect(at::TensorList ts, bool written) {
   Grads g;
   TORCH_CHECK_VALUE(!ts.empty(), "grad norm: no tensors");
   for (const at::Tensor& t : ts)
     TORCH_CHECK_VALUE(t.is_cuda() && t.layout() == at::kStrided &&
-                          float_type(t) && t.device() == ts[0].device(),
+                          float_type(t.scalar_type()) && t.device() == ts[0].device(),
                       "grad norm: tensors must be dense float/half/bfloat16 "
                       "on one GPU");
   // By address: equal tensors are neighbours then (of those that start at one
@@ -423,8 +540,8 @@ void write_back(const Grads& g) {
 
 // (norm, factor) as fp32[2], and the tensors scaled by the factor if `clip`;
 // type 0 is the maximum.
-at::Tensor norm_of(const std::vector<at::Tensor>& ts, int64_t type,
-                   double max_norm, bool clip) {
+at::Tensor norm_of(at::TensorList ts, int64_t type, double max_norm,
+                   bool clip) {
   TORCH_CHECK(type >= 0 && type <= 2, "grad norm: type");
   const Grads g = collect(ts, clip);
   const Guard guard(ts[0].device());
@@ -461,9 +578,16 @@ at::Tensor norm_of(const std::vector<at::Tensor>& ts, int64_t type,
   return out;
 }
 
+at::Tensor grad_norm_kernel(at::TensorList ts, int64_t type,
+                            double max_norm) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  return norm_of(ts, type, max_norm, false);
+}
+
 at::Tensor grad_norm(const std::vector<at::Tensor>& ts, int64_t type,
                      double max_norm) {
-  return norm_of(ts, type, max_norm, false);
+  static const auto op = op_of<decltype(grad_norm_kernel)>("axon::grad_norm");
+  return op.call(ts, type, max_norm);
 }
 
 // The gradients of lists of parameters, read here rather than in Python:
@@ -478,7 +602,7 @@ bool param_grads(const pybind11::list& lists, std::vector<at::Tensor>& grads) {
       if (!THPVariable_Check(o)) return false;
       const at::Tensor& g = THPVariable_Unpack(o).grad();
       if (!g.defined()) continue;
-      if (!g.is_cuda() || g.layout() != at::kStrided || !float_type(g) ||
+      if (!g.is_cuda() || g.layout() != at::kStrided || !float_type(g.scalar_type()) ||
           (!grads.empty() && g.device() != grads[0].device()))
         return false;
       grads.push_back(g);
@@ -491,6 +615,7 @@ bool param_grads(const pybind11::list& lists, std::vector<at::Tensor>& grads) {
 // gradient, False where the general path has to take them.
 pybind11::object param_grad_norm(const pybind11::list& lists, int64_t type,
                                  double max_norm, bool clip) {
+  check_untraced("gradient clipping");
   std::vector<at::Tensor> grads;
   if (!param_grads(lists, grads)) return pybind11::bool_(false);
   if (grads.empty()) return pybind11::none();
@@ -498,6 +623,7 @@ pybind11::object param_grad_norm(const pybind11::list& lists, int64_t type,
 }
 
 void grad_scale_(const std::vector<at::Tensor>& ts, const at::Tensor& factor) {
+  check_untraced("gradient clipping");
   const Grads g = collect(ts, true);
   TORCH_CHECK(factor.device() == ts[0].device() && factor.numel() == 1 &&
                   factor.scalar_type() == at::kFloat,
@@ -508,6 +634,34 @@ void grad_scale_(const std::vector<at::Tensor>& ts, const at::Tensor& factor) {
                       stream_of(ts[0]));
   write_back(g);
   check_launch();
+}
+
+TORCH_LIBRARY(axon, m) {
+  m.def("embedding(Tensor ids, Tensor weight, float scale, int? padding_idx) "
+        "-> Tensor");
+  m.def("embedding_backward(Tensor ids, Tensor grad, int vocab, int padding, "
+        "float scale) -> Tensor");
+  m.def("cross_entropy(Tensor logits, Tensor target, int ignore_index, "
+        "float label_smoothing, int reduction) -> (Tensor, Tensor)");
+  m.def("cross_entropy_backward(Tensor grad, Tensor logits, Tensor target, "
+        "Tensor kept, int ignore_index, float label_smoothing, int reduction) "
+        "-> Tensor");
+  m.def("grad_norm(Tensor[] tensors, int norm_type, float max_norm) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(axon, CUDA, m) {
+  m.impl("embedding", &embedding_kernel);
+  m.impl("embedding_backward", &embedding_backward_kernel);
+  m.impl("cross_entropy", &cross_entropy_kernel);
+  m.impl("cross_entropy_backward", &cross_entropy_backward_kernel);
+  m.impl("grad_norm", &grad_norm_kernel);
+}
+
+TORCH_LIBRARY_IMPL(axon, AutogradCUDA, m) {
+  m.impl("embedding", &embedding_autograd);
+  m.impl("cross_entropy", &cross_entropy_autograd);
+  // Its callers compute it without gradients.
+  m.impl("grad_norm", torch::CppFunction::makeFallthrough());
 }
 
 }  // namespace

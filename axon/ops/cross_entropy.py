@@ -22,7 +22,7 @@ def cross_entropy(logits, target, ignore_index=-100, label_smoothing=0.0,
     and its row's gradient NaN (a check would wait for the GPU); on the CPU it
     raises IndexError. A call on the GPU takes up to 2^24 - 256 rows, 2^26 -
     256 of up to 1024 vectors of 16 bytes. The gradient is not differentiable
-    again.
+    again. A trace holds the call as the operator axon::cross_entropy.
     """
     if logits.is_cuda and logits.dtype in _SUPPORTED:
         from axon import _core

@@ -20,7 +20,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     On the GPU an id outside [0, V) gives a row of NaN and no gradient (a
     check would wait for the GPU); on the CPU it raises IndexError. A call on
     the GPU takes fewer than 2^26 ids. The gradient is not differentiable
-    again.
+    again. A trace holds the call as the operator axon::embedding.
     """
     if isinstance(scale, torch.Tensor):
         raise TypeError("embedding: scale must be a number")

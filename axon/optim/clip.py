@@ -87,7 +87,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0,
     once and is scaled once; on the GPU, gradients that share memory in part
     are refused.
     A norm of inf or NaN makes the factor 0 or NaN as in torch;
-    error_if_nonfinite raises instead (and waits for the GPU).
+    error_if_nonfinite raises instead (and waits for the GPU). On the GPU a
+    call cannot be traced (NotImplementedError): the gradients are no arguments.
 
     Under DistributedOptimizer the gradients are averaged first:
 
