@@ -615,10 +615,10 @@ bool param_grads(const pybind11::list& lists, std::vector<at::Tensor>& grads) {
 // gradient, False where the general path has to take them.
 pybind11::object param_grad_norm(const pybind11::list& lists, int64_t type,
                                  double max_norm, bool clip) {
-  check_untraced("gradient clipping");
   std::vector<at::Tensor> grads;
   if (!param_grads(lists, grads)) return pybind11::bool_(false);
   if (grads.empty()) return pybind11::none();
+  check_untraced("gradient clipping");
   return pybind11::cast(norm_of(grads, type, max_norm, clip));
 }
 
