@@ -114,6 +114,8 @@ class BertForPreTraining(nn.Module):
         return h @ self.tok.weight.t() + self.mlm_bias
 
     def mlm_loss(self, input_ids, labels, **kw):
-        """labels = -100 where not masked (standard MLM convention)."""
-        return cross_entropy(self.forward(input_ids, **kw), labels,
+        """labels = -100 where not masked (standard MLM convention); as many
+        as input_ids, in any shape."""
+        return cross_entropy(self.forward(input_ids, **kw),
+                             labels.reshape(input_ids.shape),
                              ignore_index=-100)
