@@ -42,13 +42,15 @@ def _once(tensors):
 
 
 def _norm_eager(tensors, norm_type):
-    norms = [torch.linalg.vector_norm(t.detach().double(), norm_type)
+    norms = [torch.linalg.vector_norm(
+                 t.detach().to(torch.complex128 if t.is_complex()
+                               else torch.float64), norm_type)
              for t in _once(tensors) if t.numel()]
     if not norms:
         return torch.zeros((), device=tensors[0].device)
     norms = torch.stack([n.to(norms[0].device) for n in norms])
     total = torch.linalg.vector_norm(norms, norm_type)
-    wide = any(t.dtype == torch.float64 for t in tensors)
+    wide = any(t.dtype in (torch.float64, torch.complex128) for t in tensors)
     return total if wide else total.float()
 
 

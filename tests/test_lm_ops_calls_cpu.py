@@ -27,3 +27,29 @@ def test_mlm_loss_takes_flat_labels():
         assert torch.equal(model.mlm_loss(ids, flat), want)
     with pytest.raises((ValueError, RuntimeError)):
         model.mlm_loss(ids, labels[:1])
+
+
+@pytest.mark.parametrize("kind", [1.0, 2.0, float("inf")])
+def test_norm_of_complex_gradients(kind):
+    """The norm of the absolute values, and gradients scaled by it."""
+    from axon.optim import clip_grad_norm_, grad_norm
+
+    torch.manual_seed(1)
+    z = torch.randn(30, dtype=torch.complex64)
+    x = torch.randn(7)
+    size = torch.cat([z.to(torch.complex128).abs(), x.double().abs()])
+    want = torch.linalg.vector_norm(size, kind)
+    # 64-bit sums (and square roots); one rounding to fp32.
+    assert abs(grad_norm([z, x], kind).double() - want) <= 2.0 ** -23 * want
+    assert grad_norm([z, x], kind).dtype == torch.float32
+    assert grad_norm([z.to(torch.complex128)], kind).dtype == torch.float64
+    p, q = torch.nn.Parameter(z.clone()), torch.nn.Parameter(x.clone())
+    p.grad, q.grad = z.clone(), x.clone()
+    clip_grad_norm_([p, q], 0.5, kind)
+    factor = 0.5 / (want + 1e-6)
+    # The factor's rounding to fp32, the product's: 2 u each, twice for the
+    # complex one's parts.
+    for got, start in ((p.grad, z), (q.grad, x)):
+        wide = start.to(torch.complex128)
+        assert ((got.to(torch.complex128) - wide * factor).abs()
+                <= 8 * 2.0 ** -24 * wide.abs() * factor).all()
