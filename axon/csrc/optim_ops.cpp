@@ -238,6 +238,9 @@ bool fused_adam_group(pybind11::object params, pybind11::object state,
                       c10::optional<at::Tensor> grad_scale) {
   AdamLists l;
   if (!read_adam_group(params.ptr(), state.ptr(), l)) return false;
+  // The factor is where the first gradient of all groups is.
+  if (grad_scale.has_value() && !l.ps.empty())
+    grad_scale = grad_scale->to(l.ps[0].device());
   // One launch for each type and step count, in the order of the parameters.
   std::vector<std::pair<at::ScalarType, float>> keys;
   std::vector<AdamLists> parts;
