@@ -30,15 +30,18 @@ struct ChunkPlan {
   int nchunks = 0;
 };
 
+void check_type(const at::Tensor& p) {
+  TORCH_CHECK(p.scalar_type() == at::kFloat || p.scalar_type() == at::kHalf ||
+                  p.scalar_type() == at::kBFloat16,
+              "fused optimizer: float/half/bfloat16 parameters only");
+}
+
 ChunkPlan build_chunks(const std::vector<at::Tensor>& ps,
                        const std::vector<at::Tensor>& gs,
                        const std::vector<at::Tensor>& ms,
                        const std::vector<at::Tensor>& vs,
                        float* u_base /* fp32 scratch or null */) {
-  TORCH_CHECK(ps[0].scalar_type() == at::kFloat ||
-                  ps[0].scalar_type() == at::kHalf ||
-                  ps[0].scalar_type() == at::kBFloat16,
-              "fused optimizer: float/half/bfloat16 parameters only");
+  check_type(ps[0]);
   int64_t total = 0;
   for (auto& p : ps) total += p.numel();
   int64_t ce = pick_chunk_elems(total);
@@ -239,8 +242,10 @@ bool fused_adam_group(pybind11::object params, pybind11::object state,
   AdamLists l;
   if (!read_adam_group(params.ptr(), state.ptr(), l)) return false;
   // The factor is where the first gradient of all groups is.
-  if (grad_scale.has_value() && !l.ps.empty())
+  if (grad_scale.has_value() && !l.ps.empty()) {
     grad_scale = grad_scale->to(l.ps[0].device());
+    scale_ptr(grad_scale, l.ps[0]);  // refused before a step is counted
+  }
   // One launch for each type and step count, in the order of the parameters.
   std::vector<std::pair<at::ScalarType, float>> keys;
   std::vector<AdamLists> parts;
@@ -276,9 +281,25 @@ bool fused_adam_group(pybind11::object params, pybind11::object state,
   return true;
 }
 
+// Refuses a step over lists of parameters, before any of it is done, if the
+// kernels do not take one of those on a GPU that have a gradient.
+void check_fused_step(const pybind11::list& lists) {
+  for (const auto& list : lists) {
+    const pybind11::list params(  // the same one, if it is a list
+        pybind11::reinterpret_borrow<pybind11::object>(list));
+    for (size_t i = 0; i < params.size(); ++i) {
+      PyObject* o = PyList_GET_ITEM(params.ptr(), i);
+      if (!THPVariable_Check(o)) continue;
+      const at::Tensor& p = THPVariable_Unpack(o);
+      if (p.is_cuda() && p.grad().defined()) check_type(p);
+    }
+  }
+}
+
 }  // namespace
 
 void register_optim(pybind11::module_& m) {
+  m.def("check_fused_step", &check_fused_step, pybind11::arg("lists"));
   m.def("fused_adam_group", &fused_adam_group, pybind11::arg("params"),
         pybind11::arg("state"), pybind11::arg("kind"), pybind11::arg("lr"),
         pybind11::arg("beta1"), pybind11::arg("beta2"), pybind11::arg("eps"),

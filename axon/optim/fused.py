@@ -45,15 +45,16 @@ class _Clipping(Optimizer):
     def __getstate__(self):
         return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
 
-    def _clip_factor(self):
-        """The factor for this step, or None."""
-        if self.max_grad_norm is None:
-            return None
+    def _begin_step(self):
+        """Refuses what the kernels do not take, with nothing changed yet;
+        returns the factor for this step, or None."""
         from axon import _core
 
-        out = _core.param_grad_norm(
-            [group["params"] for group in self.param_groups], 2,
-            self.max_grad_norm, False)
+        lists = [group["params"] for group in self.param_groups]
+        _core.check_fused_step(lists)
+        if self.max_grad_norm is None:
+            return None
+        out = _core.param_grad_norm(lists, 2, self.max_grad_norm, False)
         if out is None:  # no gradients
             return None
         if out is not False:
@@ -105,7 +106,7 @@ class FusedSGD(_Clipping):
                 loss = closure()
         from axon import _core
 
-        factor = self._clip_factor()
+        factor = self._begin_step()
         for group in self.param_groups:
             work = []
             mu = group["momentum"]
@@ -182,7 +183,7 @@ class _FusedAdamBase(_Clipping):
                 loss = closure()
         from axon import _core
 
-        factor = self._clip_factor()
+        factor = self._begin_step()
         for group in self.param_groups:
             b1, b2 = group["betas"]
             # The steady state, in one call; False (and nothing done) where
@@ -281,7 +282,7 @@ class FusedLAMB(_Clipping):
                 loss = closure()
         from axon import _core
 
-        factor = self._clip_factor()
+        factor = self._begin_step()
         for group in self.param_groups:
             b1, b2 = group["betas"]
             if _core.fused_adam_group(group["params"], self.state, 2,

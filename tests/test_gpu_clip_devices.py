@@ -46,3 +46,41 @@ def test_groups_on_two_devices(name, first):
         assert (p - q.cpu()).abs().max() <= 3 * 0.05 * 4 * 1e-4 + 1e-6
         if name != "SGD":
             assert float(two.state[q]["step"]) == 3.0
+
+
+@pytest.mark.parametrize("clip", [None, 0.5])
+@pytest.mark.parametrize("name", ["SGD", "Adam", "AdamW", "LAMB"])
+def test_a_refused_step_changes_nothing(name, clip):
+    """A parameter that no kernel takes, behind others that are fine: before
+    and after the state is there."""
+    import axon.optim
+
+    kw = dict(momentum=0.9) if name == "SGD" else {}
+    ps = [torch.nn.Parameter(torch.ones(5, device=DEV, dtype=t))
+          for t in (torch.float32, torch.bfloat16, torch.float64)]
+    opt = getattr(axon.optim, "Fused" + name)(
+        [{"params": ps[:1]}, {"params": ps[1:]}], lr=0.1, max_grad_norm=clip,
+        **kw)
+
+    def refused():
+        for p in ps:
+            p.grad = torch.full_like(p, 0.25)
+        before = [p.detach().clone() for p in ps]
+        state = {p: {k: v.clone() for k, v in s.items()}
+                 for p, s in opt.state.items()}
+        with pytest.raises(RuntimeError, match="bfloat16 parameters only"):
+            opt.step()
+        assert all(torch.equal(p, b) for p, b in zip(ps, before))
+        assert set(opt.state) == set(state)
+        for p, s in state.items():
+            assert set(opt.state[p]) == set(s)
+            assert all(torch.equal(opt.state[p][k], v) for k, v in s.items())
+
+    refused()
+    for p in ps[:2]:
+        p.grad = torch.full_like(p, 0.25)
+    ps[2].grad = None
+    opt.step()
+    opt.step()
+    assert not torch.equal(ps[0].detach(), torch.ones(5, device=DEV))
+    refused()
