@@ -39,8 +39,8 @@ void check_type(const at::Tensor& p) {
 ChunkPlan build_chunks(const std::vector<at::Tensor>& ps,
                        const std::vector<at::Tensor>& gs,
                        const std::vector<at::Tensor>& ms,
-                       const std::vector<at::Tensor>& vs,
-                       float* u_base /* fp32 scratch or null */) {
+                       const std::vector<at::Tensor>& vs, bool with_m,
+                       bool with_v, float* u_base /* fp32 scratch or null */) {
   check_type(ps[0]);
   int64_t total = 0;
   for (auto& p : ps) total += p.numel();
@@ -48,20 +48,33 @@ ChunkPlan build_chunks(const std::vector<at::Tensor>& ps,
   std::vector<OptChunk> chunks;
   chunks.reserve(ps.size() + total / ce);
   int64_t uoff = 0;
+  TORCH_CHECK(gs.size() == ps.size() && ms.size() == (with_m ? ps.size() : 0) &&
+                  vs.size() == (with_v ? ps.size() : 0),
+              "fused optimizer: as many grads and states as params");
   for (size_t t = 0; t < ps.size(); ++t) {
     auto& p = ps[t];
     // Elementwise over dense storage: any non-overlapping-and-dense layout
     // (incl. channels_last) works as long as param/grad/state agree on
     // strides — same storage index = same logical element on all of them.
+    // All of one type, which the kernels read and write them as.
+    TORCH_CHECK(p.scalar_type() == ps[0].scalar_type() &&
+                    p.device() == ps[0].device(),
+                "fused optimizer: params of one type on one device");
     TORCH_CHECK(p.is_non_overlapping_and_dense() &&
                     gs[t].is_non_overlapping_and_dense(),
                 "fused optimizer requires dense params/grads");
-    TORCH_CHECK(p.numel() <= 1 || gs[t].strides() == p.strides(),
-                "fused optimizer: grad layout must match param layout");
-    TORCH_CHECK(ms.empty() || p.numel() <= 1 || ms[t].strides() == p.strides(),
-                "fused optimizer: state layout must match param layout");
-    TORCH_CHECK(vs.empty() || p.numel() <= 1 || vs[t].strides() == p.strides(),
-                "fused optimizer: state layout must match param layout");
+    for (auto* l : {&gs, &ms, &vs}) {
+      if (l->empty()) continue;
+      const at::Tensor& o = (*l)[t];
+      TORCH_CHECK(o.sizes() == p.sizes() &&
+                      o.scalar_type() == p.scalar_type() &&
+                      o.device() == p.device(),
+                  "fused optimizer: grad and state must have the param's "
+                  "shape, type and device");
+      TORCH_CHECK(p.numel() <= 1 || o.strides() == p.strides(),
+                  "fused optimizer: grad and state layout must match param "
+                  "layout");
+    }
     size_t esize = p.element_size();
     char* pp = static_cast<char*>(p.data_ptr());
     char* gg = static_cast<char*>(gs[t].data_ptr());
@@ -122,7 +135,7 @@ void fused_sgd(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                c10::optional<at::Tensor> grad_scale) {
   if (ps.empty()) return;
   auto plan = build_chunks(ps, gs, momentum != 0 ? ms : std::vector<at::Tensor>{},
-                           {}, nullptr);
+                           {}, momentum != 0, false, nullptr);
   // momentum==0 passes ms pointers as null via empty list; kernel ignores m.
   if (momentum != 0) {
     TORCH_CHECK(ms.size() == ps.size(), "momentum buffers missing");
@@ -140,7 +153,7 @@ void fused_adam(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
                 int64_t step, bool adamw,
                 c10::optional<at::Tensor> grad_scale) {
   if (ps.empty()) return;
-  auto plan = build_chunks(ps, gs, ms, vs, nullptr);
+  auto plan = build_chunks(ps, gs, ms, vs, true, true, nullptr);
   float bc1 = 1.0f - std::pow(static_cast<float>(beta1), static_cast<float>(step));
   float bc2_sqrt =
       std::sqrt(1.0f - std::pow(static_cast<float>(beta2), static_cast<float>(step)));
@@ -162,7 +175,7 @@ void fused_lamb(std::vector<at::Tensor> ps, std::vector<at::Tensor> gs,
   at::Tensor u = at::empty({total}, ps[0].options().dtype(at::kFloat));
   at::Tensor norms = at::zeros({2 * static_cast<int64_t>(ps.size())},
                                ps[0].options().dtype(at::kFloat));
-  auto plan = build_chunks(ps, gs, ms, vs, static_cast<float*>(u.data_ptr()));
+  auto plan = build_chunks(ps, gs, ms, vs, true, true, static_cast<float*>(u.data_ptr()));
   float bc1 = 1.0f - std::pow(static_cast<float>(beta1), static_cast<float>(step));
   float bc2_sqrt =
       std::sqrt(1.0f - std::pow(static_cast<float>(beta2), static_cast<float>(step)));

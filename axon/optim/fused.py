@@ -12,12 +12,25 @@ def _like_param(p, t):
     param's strides (channels_last params included). Autograd or a loaded
     checkpoint can hand us a differently-laid-out tensor — restride it once.
     Grads are read-only in the kernels, so a copy is safe."""
+    if p.is_cuda and t is not None and (t.dtype != p.dtype or
+                                        t.shape != p.shape or
+                                        t.device != p.device):
+        raise RuntimeError(
+            "fused optimizer: gradient or state "
+            f"({t.dtype}, {tuple(t.shape)}, {t.device}) of a parameter "
+            f"({p.dtype}, {tuple(p.shape)}, {p.device}); state of a model that "
+            "was cast or moved: opt.load_state_dict(opt.state_dict())")
     if t is None or p.numel() <= 1 or t.stride() == p.stride():
         return t
     out = torch.empty_strided(p.shape, p.stride(), dtype=t.dtype,
                               device=t.device)
     out.copy_(t)
     return out
+
+
+def _next_step(step):
+    step += 1
+    return int(step.item())
 
 
 def _grouped(params_with_grad):
@@ -202,11 +215,12 @@ class _FusedAdamBase(_Clipping):
                     st["step"] = torch.tensor(0.0)
                     st["exp_avg"] = torch.zeros_like(p)
                     st["exp_avg_sq"] = torch.zeros_like(p)
-                st["step"] += 1
                 st["exp_avg"] = _like_param(p, st["exp_avg"])
                 st["exp_avg_sq"] = _like_param(p, st["exp_avg_sq"])
                 work.append((p, _like_param(p, p.grad), st["exp_avg"],
-                             st["exp_avg_sq"], int(st["step"].item())))
+                             st["exp_avg_sq"], st["step"]))
+            # Counted once all of the group has been looked over.
+            work = [t[:4] + (_next_step(t[4]),) for t in work]
             for tuples in _grouped(work):
                 # all params in a (device,dtype) bucket share the step count
                 # only if they were created together; split by step to be safe
@@ -298,11 +312,12 @@ class FusedLAMB(_Clipping):
                     st["step"] = torch.tensor(0.0)
                     st["exp_avg"] = torch.zeros_like(p)
                     st["exp_avg_sq"] = torch.zeros_like(p)
-                st["step"] += 1
                 st["exp_avg"] = _like_param(p, st["exp_avg"])
                 st["exp_avg_sq"] = _like_param(p, st["exp_avg_sq"])
                 work.append((p, _like_param(p, p.grad), st["exp_avg"],
-                             st["exp_avg_sq"], int(st["step"].item())))
+                             st["exp_avg_sq"], st["step"]))
+            # Counted once all of the group has been looked over.
+            work = [t[:4] + (_next_step(t[4]),) for t in work]
             for tuples in _grouped(work):
                 by_step = {}
                 for t in tuples:

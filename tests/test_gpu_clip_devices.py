@@ -84,3 +84,60 @@ def test_a_refused_step_changes_nothing(name, clip):
     opt.step()
     assert not torch.equal(ps[0].detach(), torch.ones(5, device=DEV))
     refused()
+
+
+@pytest.mark.parametrize("name", ["SGD", "Adam", "AdamW", "LAMB"])
+@pytest.mark.parametrize("now", [torch.float32, torch.float16])
+def test_state_of_another_type_is_refused(name, now):
+    """A model cast after its optimizer's first step: the kernels read state
+    as the parameter's type, past its end if that is wider."""
+    import axon.optim
+
+    layer = torch.nn.Linear(8, 4).to(DEV, torch.bfloat16)
+    kw = dict(momentum=0.9) if name == "SGD" else {}
+    opt = getattr(axon.optim, "Fused" + name)(layer.parameters(), lr=0.1, **kw)
+    for p in layer.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    layer.to(now)
+    for p in layer.parameters():
+        p.grad = torch.ones_like(p)
+    before = [p.detach().clone() for p in layer.parameters()]
+    state = {p: {k: v.clone() for k, v in s.items()}
+             for p, s in opt.state.items()}
+    with pytest.raises(RuntimeError, match="state"):
+        opt.step()
+    assert all(torch.equal(p, b)
+               for p, b in zip(layer.parameters(), before))
+    for p, s in state.items():
+        assert all(torch.equal(opt.state[p][k], v) for k, v in s.items())
+    opt.load_state_dict(opt.state_dict())  # brings the state to the new type
+    opt.step()
+    assert all(not torch.equal(p, b)
+               for p, b in zip(layer.parameters(), before))
+
+
+def test_core_refuses_lists_that_do_not_match():
+    """The launchers themselves: state of another type, shape or device."""
+    from axon import _core
+
+    p, g = (torch.ones(4, 6, device=DEV) for _ in range(2))
+    bad = [torch.ones(4, 6, device=DEV, dtype=torch.bfloat16),
+           torch.ones(2, 6, device=DEV), torch.ones(4, 6)]
+    for m in bad:
+        for gs, ms, vs in (([m], [g], [g]), ([g], [m], [g]), ([g], [g], [m])):
+            with pytest.raises(RuntimeError, match="fused optimizer"):
+                _core.fused_adam([p], gs, ms, vs, 0.1, 0.9, 0.99, 1e-8, 0.0, 1,
+                                 False)
+            with pytest.raises(RuntimeError, match="fused optimizer"):
+                _core.fused_lamb([p], gs, ms, vs, 0.1, 0.9, 0.99, 1e-8, 0.0, 1)
+        with pytest.raises(RuntimeError, match="fused optimizer"):
+            _core.fused_sgd([p], [g], [m], 0.1, 0.9, 0.0, 0.0, False, False)
+    with pytest.raises(RuntimeError, match="fused optimizer"):
+        _core.fused_sgd([p, p], [g], [g, g], 0.1, 0.9, 0.0, 0.0, False, False)
+    with pytest.raises(RuntimeError, match="fused optimizer"):
+        _core.fused_sgd([p], [g], [], 0.1, 0.9, 0.0, 0.0, False, False)
+    with pytest.raises(RuntimeError, match="fused optimizer"):
+        _core.fused_adam([p], [g], [g], [], 0.1, 0.9, 0.99, 1e-8, 0.0, 1,
+                         False)
+    assert torch.equal(p, torch.ones(4, 6, device=DEV))
