@@ -55,12 +55,18 @@ void check_launch() {
               hipGetErrorString(e));
 }
 
-// A gradient that must not be differentiated again, under create_graph.
-at::Tensor once(at::Tensor grad, const char* what) {
-  if (!at::GradMode::is_enabled()) return grad;
-  auto f = std::make_shared<torch::autograd::DelayedError>(
-      std::string(what) + ": the gradient is not differentiable again", 1);
-  return (*f)({std::move(grad)})[0];
+// A gradient that must not be differentiated again: an error where that is
+// tried, under torch's graph as under its function transforms.
+template <typename... Inputs>
+at::Tensor once(at::Tensor grad, const char* what, const Inputs&... inputs) {
+  if (!torch::autograd::compute_requires_grad(inputs...)) return grad;
+  auto node = std::shared_ptr<torch::autograd::Error>(
+      new torch::autograd::Error(
+          std::string(what) + ": the gradient is not differentiable again",
+          torch::autograd::collect_next_edges(inputs...)),
+      torch::autograd::deleteNode);
+  torch::autograd::set_history(grad, node);
+  return grad;
 }
 
 // Forward-mode tangents would be lost without a word.
@@ -176,6 +182,25 @@ at::Tensor embedding_backward_kernel(const at::Tensor& ids_in,
   return dw;
 }
 
+at::Tensor embedding_backward(const at::Tensor& ids, const at::Tensor& dy,
+                              int64_t vocab, int64_t padding, double scale) {
+  static const auto op = op_of<decltype(embedding_backward_kernel)>(
+      "axon::embedding_backward");
+  return op.call(ids, dy, vocab, padding, scale);
+}
+
+at::Tensor embedding_backward_autograd(const at::Tensor& ids,
+                                       const at::Tensor& dy, int64_t vocab,
+                                       int64_t padding, double scale) {
+  check_no_tangent(dy, "embedding");
+  at::Tensor dw;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    dw = embedding_backward(ids, dy, vocab, padding, scale);
+  }
+  return once(dw, "embedding", dy);
+}
+
 struct EmbeddingBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable ids;
   int64_t vocab = 0, padding = -1;
@@ -183,17 +208,10 @@ struct EmbeddingBackward : public torch::autograd::Node {
 
   torch::autograd::variable_list apply(
       torch::autograd::variable_list&& grads) override {
-    static const auto op = op_of<decltype(embedding_backward_kernel)>(
-        "axon::embedding_backward");
     std::lock_guard<std::mutex> lock(mutex_);
     const at::Tensor i = ids.unpack(shared_from_this());
     if (!grads[0].defined()) return {at::Tensor()};
-    at::Tensor dw;
-    {
-      at::AutoDispatchBelowADInplaceOrView below;
-      dw = op.call(i, grads[0], vocab, padding, scale);
-    }
-    return {once(dw, "embedding")};
+    return {embedding_backward(i, grads[0], vocab, padding, scale)};
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -351,6 +369,30 @@ at::Tensor cross_entropy_backward_kernel(
   return dx;
 }
 
+at::Tensor cross_entropy_backward(const at::Tensor& grad,
+                                  const at::Tensor& logits,
+                                  const at::Tensor& target,
+                                  const at::Tensor& kept, int64_t ignore,
+                                  double eps, int64_t reduction) {
+  static const auto op = op_of<decltype(cross_entropy_backward_kernel)>(
+      "axon::cross_entropy_backward");
+  return op.call(grad, logits, target, kept, ignore, eps, reduction);
+}
+
+at::Tensor cross_entropy_backward_autograd(
+    const at::Tensor& grad, const at::Tensor& logits, const at::Tensor& target,
+    const at::Tensor& kept, int64_t ignore, double eps, int64_t reduction) {
+  for (const at::Tensor* t : {&grad, &logits})
+    check_no_tangent(*t, "cross_entropy");
+  at::Tensor dx;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    dx = cross_entropy_backward(grad, logits, target, kept, ignore, eps,
+                                reduction);
+  }
+  return once(dx, "cross_entropy", grad, logits);
+}
+
 struct CrossEntropyBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable logits, target;
   at::Tensor kept;  // of this file alone
@@ -360,17 +402,11 @@ struct CrossEntropyBackward : public torch::autograd::Node {
 
   torch::autograd::variable_list apply(
       torch::autograd::variable_list&& grads) override {
-    static const auto op = op_of<decltype(cross_entropy_backward_kernel)>(
-        "axon::cross_entropy_backward");
     std::lock_guard<std::mutex> lock(mutex_);
     const at::Tensor x = logits.unpack(), t = target.unpack();
     if (!grads[0].defined()) return {at::Tensor()};
-    at::Tensor dx;
-    {
-      at::AutoDispatchBelowADInplaceOrView below;
-      dx = op.call(grads[0], x, t, kept, ignore, eps, reduction);
-    }
-    return {once(dx, "cross_entropy")};
+    return {cross_entropy_backward(grads[0], x, t, kept, ignore, eps,
+                                   reduction)};
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -660,6 +696,8 @@ TORCH_LIBRARY_IMPL(axon, CUDA, m) {
 TORCH_LIBRARY_IMPL(axon, AutogradCUDA, m) {
   m.impl("embedding", &embedding_autograd);
   m.impl("cross_entropy", &cross_entropy_autograd);
+  m.impl("embedding_backward", &embedding_backward_autograd);
+  m.impl("cross_entropy_backward", &cross_entropy_backward_autograd);
   // Its callers compute it without gradients.
   m.impl("grad_norm", torch::CppFunction::makeFallthrough());
 }

@@ -164,3 +164,56 @@ def test_function_transforms():
     leaf = w.clone().requires_grad_()
     embedding(ids, leaf, scale=2.0).square().sum().backward()
     assert torch.equal(got, leaf.grad)
+
+
+def test_second_derivatives_are_refused():
+    """Under torch's graph and under its function transforms: an error, never
+    zeros. What does not depend on the gradient again is no error."""
+    from axon.ops import cross_entropy, embedding
+
+    x, t = _values(0, (6, 9)), _ids(0, (6,), 9)
+    w, ids = _values(1, (20, 9)), _ids(1, (6,), 20)
+
+    def loss(v):
+        return cross_entropy(v, t)
+
+    def cubes(v):
+        return embedding(ids, v).pow(3).sum()
+
+    grad = torch.func.grad
+    for f, v in ((loss, x), (cubes, w)):
+        with pytest.raises(RuntimeError, match="not differentiable again"):
+            grad(lambda u: grad(f)(u).square().sum())(v)
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(f, (v,), (torch.ones_like(v),))
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(grad(f), (v,), (torch.ones_like(v),))
+        leaf = v.clone().requires_grad_()
+        (g,) = torch.autograd.grad(f(leaf), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="not differentiable again"):
+            g.sum().backward()
+    dy = _values(2, (6, 9))
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda d: torch.func.vjp(
+            lambda v: embedding(ids, v), w)[1](d)[0], (dy,), (dy,))
+    leaf = w.clone().requires_grad_()
+    (g,) = torch.autograd.grad(embedding(ids, leaf), leaf, dy,
+                               create_graph=True)
+    assert not g.requires_grad
+
+
+def test_gradients_of_each_sample():
+    from axon.ops import cross_entropy, embedding
+
+    x, t = _values(0, (6, 9)), _ids(0, (6,), 9)
+    got = torch.func.vmap(torch.func.grad(cross_entropy))(x, t)
+    leaf = x.clone().requires_grad_()
+    cross_entropy(leaf, t, reduction="sum").backward()
+    assert torch.equal(got, leaf.grad)
+    w, ids = _values(1, (3, 20, 9)), _ids(1, (6,), 20)
+    got = torch.func.vmap(torch.func.grad(
+        lambda v: embedding(ids, v).square().sum()))(w)
+    for one, v in zip(got, w):
+        leaf = v.clone().requires_grad_()
+        embedding(ids, leaf).square().sum().backward()
+        assert torch.equal(one, leaf.grad)
