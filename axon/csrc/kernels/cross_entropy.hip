@@ -98,8 +98,8 @@ __device__ __forceinline__ float row_loss(Stat st, float xt, bool known,
 }
 
 // A group of G threads reads one segment of one row; where rows are not cut
-// (kWhole) it finishes the row as well. 8192 rows of 128256 bf16 in 301 us,
-// 7.0 TB/s: memory, and nearly arithmetic as well (an exp2 at a quarter of the
+// (kWhole) it finishes the row as well. 8192 rows of 128256 bf16 in 311 us,
+// 6.8 TB/s: memory, and nearly arithmetic as well (an exp2 at a quarter of the
 // rate and 5 other instructions for a value, 240 us). So the running maximum
 // is moved once for each vector, which costs an exp2 more for 4 or 8 values.
 template <typename T, int G, bool kSmooth, bool kWhole>
@@ -283,9 +283,9 @@ __global__ __launch_bounds__(kSumThreads) void ce_sum_kernel(
 }
 
 // The gradient of one segment of one row by a group of G threads: the logits
-// again and 1/S, no division. 8192 rows of 128256 bf16 in 767 us, 5.5 TB/s of
+// again and 1/S, no division. 8192 rows of 128256 bf16 in 773 us, 5.4 TB/s of
 // reading and writing (a copy reaches 4.9); 8192 rows of 30522 of which 15 of
-// 100 have a label in 109 us, 5.3 TB/s.
+// 100 have a label in 114 us, 5.0 TB/s.
 template <typename T, int G, bool kOnce>
 __global__ __launch_bounds__(kThreads) void ce_grad_kernel(
     const T* __restrict__ x, Rows rows, const int64_t* __restrict__ target,
@@ -379,10 +379,13 @@ __global__ __launch_bounds__(kThreads) void ce_grad_kernel(
 // 63 by waves, 100 + 118 by blocks; of 8000 162 + 369 by waves, 208 + 394 by
 // blocks; of 12000 (half as many) 120 + 279 and 125 + 263.
 //
-// Where rows are too few for two blocks on each CU, long ones are cut into
-// segments of 4096 logits or more, and joined by a launch of its own: 511 rows
-// of 32003 fp16 took 8.4 us whole, 11.3 and 12.7 in 2 and 4 segments; 64 rows
-// of 128256 8.1 us in 8 segments, 11.3 in 31.
+// Up to 256 long rows are cut into 512 / n segments, whole numbers of them, of
+// 4096 logits or more, and joined by a launch of its own; more rows stay whole.
+// 511 rows of 32003 fp16 took 8.4 us whole, 11.3 and 12.7 in 2 and 4 segments;
+// 64 rows of 128256 8.1 us in 8 segments, 11.3 in 31. As it is, a call for 64,
+// 96, 160 and 256 rows of 128256 bf16 takes 8.9, 9.6, 12.5 and 16.2 us in 8, 5, 3
+// and 2 segments, one for 257, 300, 400 and 511 whole rows 18.0, 19.5, 19.4 and
+// 21.6.
 struct Plan {
   int group;
   int segs;

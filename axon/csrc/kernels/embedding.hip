@@ -24,8 +24,8 @@ constexpr int kThreads = 256;
 //
 // A group of `lanes` lanes copies up to kFwdVecs 16-byte vectors of one row;
 // wide rows are spread over gridDim.y. 32768 rows of 4096 bf16 from a table
-// of 128256: 72 us, 5.2 TB/s (92 us right behind a gradient, whose last zeros
-// still go to memory then); 8 rows of 2048: 2.3 us, the latency of two
+// of 128256, 12549 of them different as in a text: 79 us, 4.7 TB/s (91 us right
+// behind a gradient, whose last zeros still go to memory then); 8 rows of 2048: 2.3 us, the latency of two
 // dependent loads and a store. An id outside [0, V) gives a row of
 // NaN: the kernel reads nothing for it, and the caller sees it in the loss.
 
@@ -95,7 +95,7 @@ constexpr int kMergeRuns = 16;
 
 // dW is filled with zeros by further blocks of the sorting launches, which
 // leave memory idle; each writes kFillUnits units of 16 bytes. (1.05 GB of
-// zeros and the keys of 32768 tokens: 82 + 94 us, 6.0 TB/s; the keys alone take
+// zeros and the keys of 32768 tokens: 82 + 96 us, 5.9 TB/s; the keys alone take
 // 11 + 7.)
 constexpr int kFillUnits = 4096;
 
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(kMergeRuns * 64) void embed_merge_kernel(
 // from the lanes makes ids and row addresses uniform, so that changes of the
 // id are scalar branches and kRowsAhead rows are in flight. The rows of dy are
 // read once, past the caches, which are full of dW's zeros: 32768 rows of 4096
-// bf16 take 79 us (5.0 TB/s, with the rows of dW) and took 119 through them.
+// bf16 take 78 us (5.0 TB/s, with the rows of dW) and took 119 through them.
 
 constexpr int kRowsAhead = 8;
 constexpr int kMaxChunk = 64;

@@ -10,9 +10,9 @@
 // chunks b, b + grid, ... and its partial sum has a place of its own, so the
 // same gradients give the same bits.
 //
-// Measured: the norm of 1.5G bf16 values 525 us (5.7 TB/s), of 25.6M fp32
-// values 16.6 us (6.2 TB/s); the squares in 64 bits hide behind the loads. 335M
-// bf16 values in two tables: norm 139 us (4.8 TB/s), scaling 213 us (6.3 TB/s
+// Measured: the norm of 1.5G bf16 values 529 us (5.7 TB/s), of 25.6M fp32
+// values 16.0 us (6.4 TB/s); the squares in 64 bits hide behind the loads. 335M
+// bf16 values in two tables: norm 141 us (4.7 TB/s), scaling 217 us (6.2 TB/s
 // of reading and writing).
 #include <algorithm>
 
