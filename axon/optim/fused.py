@@ -46,8 +46,9 @@ class _Clipping(Optimizer):
     """max_grad_norm: step() first takes the norm over the gradients of ALL
     groups, and the fused kernels multiply each gradient by the clipping
     factor as they read it (p.grad itself stays as it is). grad_norm is the
-    last step's norm, a 0-dim tensor. Not part of the state dict, which stays
-    the stock optimizers'; copies and pickles keep it."""
+    last step's norm, a 0-dim tensor (None if it had no gradients). Not part
+    of the state dict, which stays the stock optimizers'; copies and pickles
+    keep max_grad_norm."""
     max_grad_norm = None
     grad_norm = None
 
@@ -65,6 +66,7 @@ class _Clipping(Optimizer):
 
         lists = [group["params"] for group in self.param_groups]
         _core.check_fused_step(lists)
+        self.grad_norm = None
         if self.max_grad_norm is None:
             return None
         out = _core.param_grad_norm(lists, 2, self.max_grad_norm, False)

@@ -53,3 +53,19 @@ def test_norm_of_complex_gradients(kind):
         wide = start.to(torch.complex128)
         assert ((got.to(torch.complex128) - wide * factor).abs()
                 <= 8 * 2.0 ** -24 * wide.abs() * factor).all()
+
+
+@pytest.mark.parametrize("name", ["SGD", "Adam", "AdamW", "LAMB"])
+def test_norm_of_a_step_without_gradients(name):
+    """There is none, and not an earlier step's."""
+    import axon.optim
+
+    p = torch.nn.Parameter(torch.ones(4))
+    opt = getattr(axon.optim, "Fused" + name)([p], lr=0.1, max_grad_norm=1.0)
+    p.grad = torch.ones(4)
+    opt.step()
+    assert float(opt.grad_norm) == 2.0
+    opt.zero_grad(set_to_none=True)
+    before = p.detach().clone()
+    opt.step()
+    assert opt.grad_norm is None and torch.equal(p.detach(), before)
