@@ -217,3 +217,43 @@ def test_gradients_of_each_sample():
         leaf = v.clone().requires_grad_()
         embedding(ids, leaf).square().sum().backward()
         assert torch.equal(one, leaf.grad)
+
+
+def test_modes_and_hooks_around_the_calls():
+    """Clipping in an fx trace is refused; a mode that only watches, saved
+    tensors on the CPU and recomputed ones change nothing."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.checkpoint import checkpoint
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from axon.ops import cross_entropy, embedding
+    from axon.optim import FusedAdamW, clip_grad_norm_
+
+    p = torch.nn.Parameter(torch.zeros(5, device=DEV))
+    p.grad = torch.ones(5, device=DEV)
+    opt = FusedAdamW([p], max_grad_norm=1.0)
+    for f in (lambda x: x + clip_grad_norm_([p], 1.0),
+              lambda x: (opt.step(), x)[1]):
+        with pytest.raises(NotImplementedError, match="traced"):
+            make_fx(f)(torch.zeros(1, device=DEV))
+    assert torch.equal(p.grad, torch.ones(5, device=DEV))
+    assert torch.equal(p.detach(), torch.zeros(5, device=DEV))
+
+    ids, w = _ids(0, (6,), 20), _values(0, (20, 9))
+    t = _ids(1, (6,), 9)
+
+    def loss(leaf):
+        return cross_entropy(embedding(ids, leaf, scale=2.0), t)
+
+    def grad(run):
+        leaf = w.clone().requires_grad_()
+        run(leaf).backward()
+        return leaf.grad
+
+    want = grad(loss)
+    assert torch.equal(grad(lambda v: checkpoint(
+        loss, v, use_reentrant=False)), want)
+    with FlopCounterMode(display=False):
+        assert torch.equal(grad(loss), want)
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.equal(grad(loss), want)
